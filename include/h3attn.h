@@ -166,6 +166,33 @@ int h3_attn_fwd_peer(const void* q, const void* k, const void* v, void* o_local,
                      int64_t q_row_stride, int64_t kv_head_stride, int64_t kv_row_stride, int64_t o_rank_rows,
                      int64_t o_head_stride, int64_t o_row_stride, float softmax_scale, int32_t* status, void* stream);
 
+/* Rotary positions over several axes (time, height, width, ...) computed from the positions. No
+ * counterpart in the reference, whose rotary embedding is a table of matrices (harness/sp_runtime.py:93-99).
+ *   pos: [s][n_axes] (pos_type: int32 or fp32), contiguous; n_axes 1..64
+ *   inv_freq: fp64 [64], radians per unit position of pair i; axis: int32 [64], the axis that turns pair i
+ *     (outside [0, n_axes): the pair keeps its values). Pair i is (x[i], x[i + 64]), as in h3_qknorm_rope_pack:
+ *       theta = pos[token][axis[i]] * inv_freq[i]
+ *       out[i] = cos*x[i] - sin*x[i+64],  out[i+64] = sin*x[i] + cos*x[i+64]     (inverse != 0: -theta)
+ *   Angles are formed in fp64 and reduced to a turn before fp32; rows are fp32 and rounded once to bf16.
+ * h3_rope_axes: x [s][n_heads][128] with any row and head strides that are multiples of 8; out may be x itself
+ *   (same strides). The inverse rotation is the gradient of the rotation.
+ * h3_qknorm_rope_pack_axes / _peer: as h3_qknorm_rope_pack / _peer with these angles in place of the table. */
+#define H3_POS_INT32 0
+#define H3_POS_FLOAT32 1
+int h3_rope_axes(const void* x, int64_t x_row_stride, int64_t x_head_stride, const void* pos, int32_t pos_type,
+                 int64_t n_axes, const double* inv_freq, const int32_t* axis, int32_t inverse, void* out,
+                 int64_t out_row_stride, int64_t out_head_stride, int64_t s, int64_t n_heads, void* stream);
+int h3_qknorm_rope_pack_axes(const void* q, const void* k, const void* v, int64_t in_row_stride, const void* pos,
+                             int32_t pos_type, int64_t n_axes, const double* inv_freq, const int32_t* axis,
+                             const void* q_weight, const void* k_weight, float eps, void* q_out, void* k_out,
+                             void* v_out, int64_t s_l, int64_t n_heads, int64_t heads_per_rank,
+                             int64_t out_rank_stride, int64_t out_head_stride, void* stream);
+int h3_qknorm_rope_pack_axes_peer(const void* q, const void* k, const void* v, int64_t in_row_stride, const void* pos,
+                                  int32_t pos_type, int64_t n_axes, const double* inv_freq, const int32_t* axis,
+                                  const void* q_weight, const void* k_weight, float eps, const uint64_t* rank_base,
+                                  int64_t n_ranks, int64_t tensor_stride, int64_t head_stride, int64_t row_offset,
+                                  int64_t s_l, int64_t n_heads, int64_t heads_per_rank, void* stream);
+
 /* Row-independent projection GEMM, bf16 in, fp32 accumulate, bf16 out:
  *   epilogue 0: c[m][n] = sum_k a[m][k] * w[n][k]                  (w has n_out rows)
  *   epilogue 1: c[m][n] = silu(a . w[n]) * (a . w[n_out + n])       (w = [gate; up], 2*n_out rows;

@@ -4,28 +4,13 @@
 //   * seq_to_head_unpack: receive-side reorder of that exchange (sp_runtime.py:71)
 //   * head_to_seq_unpack: head-major -> token-major rows ahead of out_proj (:125)
 // All traffic is 16-byte vectors; every warp touches whole 128-byte lines.
-#include "h3_ptx.cuh"
+#include "h3_rows.cuh"
 #include "h3attn.h"
 
 namespace h3 {
 namespace pack {
 
-constexpr int kD = 128;
-
-__device__ __forceinline__ void bf16x8_to_f32(const uint4& u, float* f) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-  }
-}
-__device__ __forceinline__ uint4 f32_to_bf16x8(const float* f) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(f[2 * i], f[2 * i + 1]);
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
+constexpr int kD = kHeadDim;
 
 // Per-row arithmetic of the fused pack. Lane g (0..7) of an 8-lane group holds elements
 // [8g, 8g+8) and [64+8g, 64+8g+8) of one 128-element head row, so every rotary pair
@@ -198,18 +183,10 @@ __global__ void __launch_bounds__(256) head_to_seq_unpack_kernel(const uint4* __
   }
 }
 
-static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-static int grid_for(long long work_items, int per_block, int max_blocks) {
-  long long b = (work_items + per_block - 1) / per_block;
-  if (b < 1) b = 1;
-  if (b > max_blocks) b = max_blocks;
-  return (int)b;
-}
-
 }  // namespace pack
 }  // namespace h3
 
+using namespace h3;
 using namespace h3::pack;
 
 extern "C" int h3_version(void) { return H3ATTN_VERSION; }

@@ -10,9 +10,12 @@ Reference counterparts:
   qknorm_rope_pack     ck.rms_rope_split_half_ + transposes + send reshape, sp_runtime.py:93-104, :69
   seq_to_head_unpack   receive-side permute copy, sp_runtime.py:71
   head_to_seq_unpack   transpose/reshape ahead of out_proj, sp_runtime.py:125
+Without a counterpart in the reference:
+  RopePositions, rope_axes   rotary positions over several axes (time, height, width)
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import os
@@ -90,6 +93,15 @@ def lib() -> ctypes.CDLL:
         L.h3_qknorm_rope_pack_peer.restype = ctypes.c_int
         L.h3_attn_fwd_peer.argtypes = [vp] * 5 + [i64] * 11 + [ctypes.c_float, i32p, vp]
         L.h3_attn_fwd_peer.restype = ctypes.c_int
+        L.h3_rope_axes.argtypes = [vp, i64, i64, vp, ctypes.c_int32, i64, vp, vp, ctypes.c_int32, vp, i64, i64, i64,
+                                   i64, vp]
+        L.h3_rope_axes.restype = ctypes.c_int
+        L.h3_qknorm_rope_pack_axes.argtypes = [vp, vp, vp, i64, vp, ctypes.c_int32, i64, vp, vp, vp, vp, f32, vp, vp,
+                                               vp, i64, i64, i64, i64, i64, vp]
+        L.h3_qknorm_rope_pack_axes.restype = ctypes.c_int
+        L.h3_qknorm_rope_pack_axes_peer.argtypes = [vp, vp, vp, i64, vp, ctypes.c_int32, i64, vp, vp, vp, vp, f32, vp,
+                                                    i64, i64, i64, i64, i64, i64, i64, vp]
+        L.h3_qknorm_rope_pack_axes_peer.restype = ctypes.c_int
         L.h3_copy_2d.argtypes = [vp, i64, vp, i64, i64, i64, vp]
         L.h3_copy_2d.restype = ctypes.c_int
         L.h3_status_read.argtypes = [i32p, vp]
@@ -112,6 +124,19 @@ def _cuda(t: torch.Tensor, name: str, dtype=torch.bfloat16) -> None:
         raise H3Error(f"{name} must be a CUDA tensor (this library has no CPU path)")
     if t.dtype != dtype:
         raise H3Error(f"{name} must be {dtype}, got {t.dtype}")
+
+
+def _together(dev, **tensors) -> None:
+    """Every given tensor lives on `dev`."""
+    for n, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise H3Error(f"{n} is on {t.device}, the call runs on {dev}")
+
+
+def _on(dev):
+    """Context in which `dev` is the current device: a launch goes to its tensors' device, on the
+    stream that is current there."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def status_word(device=None) -> torch.Tensor:
@@ -188,6 +213,83 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, s_kv: int | Non
     return out
 
 
+# ----------------------------------------------------------------------------- rotary positions
+def rope_axes_freqs(sections, theta: float = 10000.0, interleaved: bool = False, device=None):
+    """(inv_freq, axis) of a rotary plan over len(sections) axes for RopePositions: axis a turns sections[a]
+    of the head's 64 pairs with frequencies theta^(-j / sections[a]), j = 0, 1, ... Pairs are handed
+    out axis after axis, or pair by pair in turn when interleaved; sections may sum to less than 64, the
+    last pairs then keep their values. Made once per model."""
+    sections = [int(n) for n in sections]
+    if not 1 <= len(sections) <= 64 or min(sections) < 0 or sum(sections) > D // 2 or not theta > 0:
+        raise H3Error(f"sections must be 1 to 64 counts >= 0 that sum to at most {D // 2}, theta > 0")
+    pairs = [(j, a) for a, n in enumerate(sections) for j in range(n)]
+    if interleaved:
+        pairs.sort()
+    rest = D // 2 - len(pairs)
+    inv = [float(theta) ** (-j / sections[a]) for j, a in pairs] + [0.0] * rest
+    return (torch.tensor(inv, dtype=torch.float64, device=device),
+            torch.tensor([a for _, a in pairs] + [-1] * rest, dtype=torch.int32, device=device))
+
+
+class RopePositions:
+    """Positions of tokens on several axes and the frequencies that turn them:
+      pos: [tokens, axes] int32 or fp32; inv_freq: fp64 [64] radians per unit position of pair (i, i + 64);
+      axis: int32 [64], the axis of each pair (outside [0, axes): the pair keeps its values).
+    Accepted by qknorm_rope_pack / _peer in place of a table of rotation matrices, by rope_axes, and as
+    sp_runtime's rope_freqs."""
+
+    __slots__ = ("pos", "inv_freq", "axis")
+
+    def __init__(self, pos: torch.Tensor, inv_freq: torch.Tensor, axis: torch.Tensor):
+        self.pos, self.inv_freq, self.axis = pos, inv_freq, axis
+
+    def rows(self, lo: int, hi: int) -> "RopePositions":
+        """The positions of tokens [lo, hi); tokens past the last one (padding) sit at position 0."""
+        n = self.pos.shape[0]
+        pos = self.pos[min(lo, n):min(hi, n)]
+        if pos.shape[0] < hi - lo:
+            pos = torch.cat([pos, pos.new_zeros((hi - lo - pos.shape[0],) + tuple(pos.shape[1:]))])
+        return RopePositions(pos.contiguous(), self.inv_freq, self.axis)
+
+    def _args(self, tokens: int, dev) -> tuple:
+        """(pos, type, axes, inv_freq, axis) for the C calls, checked."""
+        pos, f, a = self.pos, self.inv_freq, self.axis
+        for n, t, dt in (("inv_freq", f, torch.float64), ("axis", a, torch.int32)):
+            _cuda(t, n, dt)
+            if tuple(t.shape) != (D // 2,) or not t.is_contiguous():
+                raise H3Error(f"{n} must be contiguous [{D // 2}]")
+        if not isinstance(pos, torch.Tensor) or pos.dtype not in (torch.int32, torch.float32):
+            raise H3Error("pos must be an int32 or fp32 tensor")
+        _cuda(pos, "pos", pos.dtype)
+        if pos.dim() != 2 or pos.shape[0] != tokens or not 1 <= pos.shape[1] <= 64 or not pos.is_contiguous():
+            raise H3Error(f"pos must be contiguous [{tokens}, axes] with 1 to 64 axes, got {tuple(pos.shape)}")
+        _together(dev, pos=pos, inv_freq=f, axis=a)
+        return pos.data_ptr(), int(pos.dtype == torch.float32), pos.shape[1], f.data_ptr(), a.data_ptr()
+
+
+def rope_axes(x: torch.Tensor, positions: RopePositions, inverse: bool = False,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotate x [tokens, heads, 128] (bf16, last dim contiguous, row and head strides multiples of 8) by
+    its tokens' positions; inverse=True applies the transposed rotation, which is the rotation's gradient.
+    out (default: a new contiguous tensor) may be x itself."""
+    _cuda(x, "x")
+    if x.dim() != 3 or x.shape[-1] != D or x.stride(-1) != 1:
+        raise H3Error(f"x must be [tokens, heads, 128] with a contiguous last dim, got {tuple(x.shape)}")
+    if out is None:
+        out = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
+    else:
+        _cuda(out, "out")
+        if out.shape != x.shape or out.stride(-1) != 1:
+            raise H3Error(f"out must be {tuple(x.shape)} with a contiguous last dim")
+        _together(x.device, out=out)
+    args = positions._args(x.shape[0], x.device)
+    with _on(x.device):
+        rc = lib().h3_rope_axes(x.data_ptr(), x.stride(0), x.stride(1), *args, int(inverse), out.data_ptr(),
+                                out.stride(0), out.stride(1), x.shape[0], x.shape[1], _stream())
+    _check(rc, "h3_rope_axes")
+    return out
+
+
 # ----------------------------------------------------------------------------- fused exchanges (peer memory)
 def qknorm_rope_pack_peer(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rope: torch.Tensor | None,
                           q_weight: torch.Tensor | None, k_weight: torch.Tensor | None, eps: float, world: int,
@@ -195,12 +297,22 @@ def qknorm_rope_pack_peer(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rop
     """The pack with the seq->head exchange fused in: head g of each token goes straight to rank
     g // (H/world)'s buffer at rank_base[rank] (int64 device tensor [world] of addresses mapped in
     this process) + tensor*tensor_stride + local_head*head_stride + (row_offset + token)*128."""
-    q2, k2, v2, sl, H, rope_ptr, rope_stride, wptr = _pack_args(q, k, v, rope, q_weight, k_weight)
+    axes = rope if isinstance(rope, RopePositions) else None
+    q2, k2, v2, sl, H, rope_ptr, rope_stride, wptr = _pack_args(q, k, v, None if axes else rope, q_weight, k_weight)
     if H % world:
         raise H3Error(f"heads {H} not divisible by world {world}")
     _cuda(rank_base, "rank_base", torch.int64)
     if tuple(rank_base.shape) != (world,) or not rank_base.is_contiguous():
         raise H3Error("rank_base must be a contiguous int64 [world] device tensor")
+    if axes is not None:
+        _together(q.device, k=k, v=v, q_weight=q_weight, k_weight=k_weight, rank_base=rank_base)
+        with _on(q.device):
+            rc = lib().h3_qknorm_rope_pack_axes_peer(
+                q2.data_ptr(), k2.data_ptr(), v2.data_ptr(), q2.stride(0), *axes._args(sl, q.device), wptr[0], wptr[1],
+                float(eps), rank_base.data_ptr(), world, tensor_stride, head_stride, row_offset, sl, H, H // world,
+                _stream())
+        _check(rc, "h3_qknorm_rope_pack_axes_peer")
+        return
     rc = lib().h3_qknorm_rope_pack_peer(q2.data_ptr(), k2.data_ptr(), v2.data_ptr(), q2.stride(0), rope_ptr,
                                         rope_stride, wptr[0], wptr[1], float(eps), rank_base.data_ptr(), world,
                                         tensor_stride, head_stride, row_offset, sl, H, H // world, _stream())
@@ -273,11 +385,12 @@ def qknorm_rope_pack(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rope: to
                      q_weight: torch.Tensor | None, k_weight: torch.Tensor | None, eps: float, world: int,
                      out: torch.Tensor | None = None, head_major: bool = False) -> torch.Tensor:
     """q, k, v: [S_l, H*128] (views of the fused QKV output are fine; rows may be strided).
-    rope: fp32 [S_l, 64, 2, 2] or None. Returns the seq->head send buffer
+    rope: fp32 [S_l, 64, 2, 2], a RopePositions over S_l tokens, or None. Returns the seq->head send buffer
     [world, 3, H/world, S_l, 128] with q and k RMS-normalised (+ rotated); head_major=True lays
     it out [H/world, world, 3, S_l, 128] instead, so each local head's blocks for all peers are
     one contiguous all-to-all buffer (head-by-head pipelining)."""
-    q2, k2, v2, sl, H, rope_ptr, rope_stride, wptr = _pack_args(q, k, v, rope, q_weight, k_weight)
+    axes = rope if isinstance(rope, RopePositions) else None
+    q2, k2, v2, sl, H, rope_ptr, rope_stride, wptr = _pack_args(q, k, v, None if axes else rope, q_weight, k_weight)
     if H % world:
         raise H3Error(f"heads {H} not divisible by world {world}")
     hl = H // world
@@ -291,6 +404,16 @@ def qknorm_rope_pack(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rope: to
     else:           # element (rank, tensor, h, row) at ((rank*3 + tensor)*hl + h)*sl + row
         tstride, rank_stride, head_stride = hl * sl * D, 3 * hl * sl * D, sl * D
     base = out.data_ptr()
+    if axes is not None:
+        _cuda(out, "out")
+        _together(q.device, k=k, v=v, q_weight=q_weight, k_weight=k_weight, out=out)
+        with _on(q.device):
+            rc = lib().h3_qknorm_rope_pack_axes(
+                q2.data_ptr(), k2.data_ptr(), v2.data_ptr(), q2.stride(0), *axes._args(sl, q.device), wptr[0], wptr[1],
+                float(eps), base, base + 2 * tstride, base + 4 * tstride, sl, H, hl, rank_stride, head_stride,
+                _stream())
+        _check(rc, "h3_qknorm_rope_pack_axes")
+        return out
     rc = lib().h3_qknorm_rope_pack(q2.data_ptr(), k2.data_ptr(), v2.data_ptr(), q2.stride(0), rope_ptr, rope_stride,
                                    wptr[0], wptr[1], float(eps), base, base + 2 * tstride, base + 4 * tstride, sl, H,
                                    hl, rank_stride, head_stride, _stream())
