@@ -40,6 +40,7 @@ extern "C" {
 #define H3_ERR_CUDA (-9)        /* a CUDA runtime call failed (h3_status_read) */
 #define H3_ERR_SCRATCH_LIMIT (-10)  /* h3_attn_layer_noalloc: the call needs more than its static scratch */
 #define H3_ERR_DEVICE_TIMEOUT (-11) /* h3_attn_layer_noalloc: a kernel gave up waiting (bounded wait) */
+#define H3_ERR_WORKSPACE (-12)      /* the workspace is smaller than the call needs */
 
 /* device status codes (positive, written by kernels into the status word) */
 #define H3_STATUS_OK 0
@@ -165,6 +166,29 @@ int h3_attn_fwd_peer(const void* q, const void* k, const void* v, void* o_local,
                      int64_t n_ranks, int64_t n_heads, int64_t s_q, int64_t s_kv, int64_t q_head_stride,
                      int64_t q_row_stride, int64_t kv_head_stride, int64_t kv_row_stride, int64_t o_rank_rows,
                      int64_t o_head_stride, int64_t o_row_stride, float softmax_scale, int32_t* status, void* stream);
+
+/* Attention with a sliding window and first tokens that stay visible, head_dim 128, bf16 in / fp32 accumulate /
+ * bf16 out. No counterpart in the reference (its attention is dense, harness/sp_runtime.py:119-121). Query row i sits
+ * at key position p = q_start + i and sees key j when
+ *     j < s_kv  and  (j < sinks  or  p - left <= j <= p + right)        causal != 0: and j <= p (right is then 0)
+ * left / right < 0: no bound on that side. A query that sees no key gets zeros. K and V may hold anything where no
+ * query looks; where one does, V must be finite (a non-finite V row can reach up to 255 neighbouring queries
+ * of the same heads that do not see it).
+ *   q: [n_heads][s_q][128], k, v: [n_kv_heads][s_kv][128] (strides as h3_attn_fwd; n_heads a multiple of n_kv_heads,
+ *   at most 128 times it; query head h reads key head h / (n_heads / n_kv_heads)); o as h3_attn_fwd. Lengths and
+ *   |q_start| up to 2^29.
+ * h3_window_attn_plan returns the number of splits of the key axis (>= 1, or an error) that h3_window_attn should be
+ * given, and the bytes of fp32 workspace (16-byte aligned, 0 for one split) that it then needs; splits = 0 lets the
+ * plan choose by the call's shape and the GPU, 1..64 fixes it. One split gives every query row the same bits whatever
+ * heads share the call. The workspace may be reused once the call's work on the stream is done. */
+int h3_window_attn_plan(int64_t n_heads, int64_t n_kv_heads, int64_t s_q, int64_t s_kv, int64_t left, int64_t right,
+                        int64_t sinks, int32_t causal, int64_t q_start, int64_t splits, int64_t* ws_bytes);
+int h3_window_attn(const void* q, const void* k, const void* v, void* o, int64_t n_heads, int64_t n_kv_heads,
+                   int64_t s_q, int64_t s_kv, int64_t q_head_stride, int64_t q_row_stride, int64_t kv_head_stride,
+                   int64_t kv_row_stride, int64_t o_rank_rows, int64_t o_rank_stride, int64_t o_head_stride,
+                   int64_t o_row_stride, float softmax_scale, int64_t left, int64_t right, int64_t sinks,
+                   int32_t causal, int64_t q_start, int64_t splits, void* workspace, int64_t ws_bytes,
+                   int32_t* status, void* stream);
 
 /* Rotary positions over several axes (time, height, width, ...) computed from the positions. No
  * counterpart in the reference, whose rotary embedding is a table of matrices (harness/sp_runtime.py:93-99).

@@ -1,0 +1,662 @@
+// Attention with a sliding window and first tokens that stay visible, head_dim 128, bf16 in, fp32
+// accumulate, grouped key heads. Query i of the call sits at key position p_i = q_start + i and sees key j when
+//   j < s_kv  and  (j < sinks  or  p_i - left <= j <= p_i + right)     (causal: and j <= p_i)
+//   o_i = sum_j softmax_j(scale q_i . k_j) v_j over those keys; a query that sees none gets zeros.
+//
+// One pass over the visible keys with a running row maximum and sum, as the full attention kernel:
+// tcgen05 S = Q K^T (SS form) and O += P V (TS form) on 128 x 128 tiles, one softmax thread per query
+// row, O rescaled only when a row maximum grew by more than 2^8, P rounded to bf16 for the second product
+// (the tensor cores' operand type: 2^-8 of a weight at most, averaged over a row's keys; the row sum keeps the
+// fp32 weights).
+//
+// Tiles: the G = n_heads / n_kv_heads query heads that share a key head are packed into the rows of a Q
+// tile (row r = position r / G, head r % G), so a key tile is read once for all of them and a few query
+// rows fill as much of the tile as they can. A CTA walks the union of its rows' keys: the first-token run
+// [0, sinks) in 128-key tiles, then the window run from its exact first key (TMA rows need no alignment), or
+// one run from key 0 where the two touch. Only tiles on a boundary are masked, by per-row bit words.
+// Keys that no row of the CTA sees are never loaded, or (behind the end of a run, inside its last
+// tile) have their V rows zeroed in shared memory before the product, so whatever a cache
+// holds there cannot reach a result through 0 * NaN.
+//
+// kTiles = 2: CTA = 256 packed rows, 12 warps, 5-stage K/V ring, one CTA per SM (the full kernel's
+// schedule). kTiles = 1: CTA = 128 packed rows, 8 warps, 2-stage ring, two CTAs per SM. Few rows split the tile
+// list over gridDim.z CTAs; each writes (O, m, l) in fp32 to the caller's workspace and join_kernel
+// combines them in a fixed order.
+#include <algorithm>
+#include <cmath>
+
+#include "h3_attn_tile.cuh"
+
+namespace h3 {
+namespace window {
+
+using namespace h3::attn;
+
+struct Params {
+  int n_heads, group, s_q, s_kv;
+  int left, right, sinks, causal, q_start;  // sinks <= s_kv; causal: right = 0
+  int tile_pos;                             // query positions per Q tile: 128 / group
+  float scale_log2;
+  __nv_bfloat16* o;
+  long long o_rank_rows, o_rank_stride, o_head_stride, o_row_stride;
+  float* part_o;  // splits > 1: [split][head][s_q][128], unnormalised; else nullptr
+  float* part_ml; // [split][head][s_q][2]: row maximum (log2 units), row sum
+  int* status;
+};
+
+// Key tiles of one CTA: a_tiles tiles of the first-token run, then the run that begins at b_start.
+struct Walk {
+  int a_tiles, a_end, b_start, b_end, n;
+  __device__ __forceinline__ int base(int j) const { return j < a_tiles ? j * kBlockN : b_start + (j - a_tiles) * kBlockN; }
+  __device__ __forceinline__ int end(int j) const { return j < a_tiles ? a_end : b_end; }
+};
+
+__device__ __forceinline__ Walk make_walk(const Params& p, int p_first, int p_last) {
+  Walk w;
+  const int lo = max(0, p_first - p.left), hi = min(p.s_kv - 1, p_last + p.right);
+  const int ns = p.causal ? max(0, min(p.sinks, p_last + 1)) : p.sinks;
+  const bool window = lo <= hi;
+  const bool joined = window && lo <= ns;
+  w.a_tiles = joined ? 0 : (ns + kBlockN - 1) / kBlockN;
+  w.a_end = ns;
+  w.b_start = joined ? 0 : lo;
+  w.b_end = joined ? max(hi + 1, ns) : hi + 1;
+  w.n = w.a_tiles + (window ? (w.b_end - w.b_start + kBlockN - 1) / kBlockN : 0);
+  return w;
+}
+
+// Bits e of a 32-key word whose keys lie in [a, b] or below n (all relative to the word's first key).
+__device__ __forceinline__ uint32_t visible_bits(int a, int b, int n) {
+  const uint32_t ge = a <= 0 ? 0xffffffffu : (a > 31 ? 0u : 0xffffffffu << a);
+  const uint32_t le = b < 0 ? 0u : (b >= 31 ? 0xffffffffu : (2u << b) - 1u);
+  const uint32_t lt = n <= 0 ? 0u : (n > 31 ? 0xffffffffu : (1u << n) - 1u);
+  return (ge & le) | lt;
+}
+
+template <int kTiles>
+struct Cfg {
+  static constexpr int kThreads = 128 + 128 * kTiles;
+  static constexpr int kStages = kTiles == 2 ? 5 : 2;
+  // Ring stages come back through kRel release barriers used round robin: release r completes once the
+  // last tile's S(r) is ready, i.e. once every MMA reading K_r and V_(r-1) has retired. The producer trails a
+  // barrier by less than one phase while 2 * kRel > kStages - 1.
+  static constexpr int kRel = kStages;
+  static constexpr int kBarQ = 0, kBarKV = 1, kBarRel = kBarKV + kStages, kBarS = kBarRel + kRel,
+                       kBarPSplit = kBarS + kTiles, kBarPLast = kBarPSplit + kTiles, kBarO = kBarPLast + kTiles,
+                       kBarDrain = kBarO + kTiles, kNumBars = kBarDrain + 1;
+  static constexpr uint32_t kOffKV = kTiles * kTileBytes;
+  static constexpr uint32_t kOffBars = kOffKV + kStages * kTileBytes;
+  static constexpr uint32_t kSmem = 1024 + kOffBars + kNumBars * 8 + 16;
+  static constexpr int kCtasPerSm = kTiles == 2 ? 1 : 2;
+  static constexpr uint32_t kCols = kTiles * 256;  // S_t [128 t, +128), O_t [128 (kTiles + t), +128)
+  // registers: the control warpgroup gives back what the softmax warpgroups (a 128-score row a thread) take
+  static constexpr int kRegsLaunch = kTiles == 2 ? 168 : 128;
+  static constexpr int kRegsControl = kTiles == 2 ? 72 : 40;
+  static constexpr int kRegsSoftmax = 216;
+  static_assert(128 * kRegsControl + 128 * kTiles * kRegsSoftmax <= kThreads * kRegsLaunch, "register split over budget");
+};
+
+constexpr int kSplitChunks = 3;  // P is handed over after 3 of its 4 32-key chunks, then the rest
+
+template <int kTiles>
+__global__ void __launch_bounds__(Cfg<kTiles>::kThreads, Cfg<kTiles>::kCtasPerSm)
+    window_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                  const __grid_constant__ CUtensorMap tmap_v, const Params p) {
+  using C = Cfg<kTiles>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBars);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kNumBars);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  auto bar = [&](int i) { return smem_u32(&bars[i]); };
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int kvh = blockIdx.y;
+  const int i0 = blockIdx.x * kTiles * p.tile_pos;  // first query position of the CTA
+  const Walk walk = make_walk(p, p.q_start + i0, p.q_start + min(i0 + kTiles * p.tile_pos, p.s_q) - 1);
+  // this CTA's share of the tile list
+  const int j_lo = int((long long)walk.n * blockIdx.z / gridDim.z);
+  const int n_kv = int((long long)walk.n * (blockIdx.z + 1) / gridDim.z) - j_lo;
+
+  if (threadIdx.x == 0) {
+    mbar_init(bar(C::kBarQ), 1);
+    for (int s = 0; s < C::kStages; ++s) mbar_init(bar(C::kBarKV + s), 1);
+    for (int r = 0; r < C::kRel; ++r) mbar_init(bar(C::kBarRel + r), 1);
+    for (int t = 0; t < kTiles; ++t) {
+      mbar_init(bar(C::kBarS + t), 1);
+      mbar_init(bar(C::kBarPSplit + t), 128);
+      mbar_init(bar(C::kBarPLast + t), 128);
+      mbar_init(bar(C::kBarO + t), 1);
+    }
+    mbar_init(bar(C::kBarDrain), 1);
+    *abort_flag = (*reinterpret_cast<volatile int*>(p.status) != 0) ? 1 : 0;
+    fence_mbar_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmap_q);
+    tma_prefetch_desc(&tmap_k);
+    tma_prefetch_desc(&tmap_v);
+  }
+  if (warp == 2) {
+    tmem_alloc(smem_u32(tmem_slot), C::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const WaitCtx ctx{abort_flag, p.status};
+  const bool run = *abort_flag == 0 && n_kv > 0;  // uniform over the CTA
+  if (warp < 4) {
+    regs_dec<C::kRegsControl>();
+    const uint32_t sq = sbase, skv = sbase + C::kOffKV;
+    if (warp == 0 && run) {
+      // ------------------------------------------------------------ TMA producer: Q, then K_0, V_0, K_1, V_1, ...
+      const bool issuer = elect_one();
+      if (issuer) {
+        const uint32_t box = 64u * 2u * uint32_t(p.group * p.tile_pos);  // rows past group * tile_pos stay unused
+        mbar_expect_tx(bar(C::kBarQ), kTiles * 2 * box);
+        for (int t = 0; t < kTiles; ++t)
+          for (int hh = 0; hh < 2; ++hh)
+            tma_load_4d(sq + t * kTileBytes + hh * kHalfBytes, &tmap_q, bar(C::kBarQ), hh * 64, 0, i0 + t * p.tile_pos, kvh);
+      }
+      __syncwarp();
+      int it = 0;
+      bool ok = true;
+      for (int j = 0; ok && j < n_kv; ++j) {
+        const int key = walk.base(j_lo + j);
+        for (int kv = 0; kv < 2; ++kv, ++it) {
+          const int st = it % C::kStages;
+          if (it >= C::kStages) {
+            // the stage's previous item (it - kStages) is free once release e has completed: K_r (item 2r) after
+            // S(r), V_r (item 2r + 1) after S(r + 1)
+            const int e = (it - C::kStages + 1) / 2;
+            if (!__all_sync(0xffffffffu,
+                            mbar_wait(bar(C::kBarRel + e % C::kRel), uint32_t(e / C::kRel) & 1u, ctx, kStatusTimeoutKV))) {
+              ok = false;
+              break;
+            }
+          }
+          if (issuer) {
+            const CUtensorMap* m = kv ? &tmap_v : &tmap_k;
+            const uint32_t dst = skv + st * kTileBytes;
+            mbar_expect_tx(bar(C::kBarKV + st), kTileBytes);
+            tma_load_3d(dst, m, bar(C::kBarKV + st), 0, key, kvh);
+            tma_load_3d(dst + kHalfBytes, m, bar(C::kBarKV + st), 64, key, kvh);
+          }
+          __syncwarp();
+        }
+      }
+      // every issued copy must land before the CTA may exit
+      if (issuer) {
+        drain_wait(bar(C::kBarQ), 0, p.status);
+        for (int st = 0; st < C::kStages; ++st) {
+          const int cnt = it / C::kStages + (st < it % C::kStages ? 1 : 0);
+          if (cnt > 0) drain_wait(bar(C::kBarKV + st), uint32_t(cnt - 1) & 1u, p.status);
+        }
+      }
+      __syncwarp();
+    } else if (warp == 1 && run) {
+      // ------------------------------------------------------------ MMA issuer (the whole warp loops, one lane issues)
+      const bool issuer = elect_one();
+      auto wait_all = [&](uint32_t b, uint32_t par, int code) -> bool {
+        return __all_sync(0xffffffffu, mbar_wait(b, par, ctx, code));
+      };
+      auto wait_full = [&](int it) -> bool {
+        return wait_all(bar(C::kBarKV + it % C::kStages), uint32_t(it / C::kStages) & 1u, kStatusTimeoutKV);
+      };
+      auto commit = [&](int b) {
+        if (issuer) mma_commit(bar(b));
+        __syncwarp();
+      };
+      auto col_o = [&](int t) { return tmem + 128u * uint32_t(kTiles + t); };
+      auto col_p = [&](int t) { return tmem + 128u * uint32_t(t) + 64u; };
+      bool ok = wait_all(bar(C::kBarQ), 0, kStatusTimeoutQ) && wait_full(0);
+      if (ok) {
+        tc_fence_after();
+        for (int t = 0; t < kTiles; ++t) {
+          if (issuer) issue_qk(tmem + 128u * t, sq + t * kTileBytes, skv);
+          __syncwarp();
+          commit(C::kBarS + t);
+        }
+      }
+      for (int j = 0; ok && j < n_kv; ++j) {
+        const int it_v = 2 * j + 1, it_k = 2 * j + 2;
+        const bool next = j + 1 < n_kv;
+        if (!(ok = wait_full(it_v))) break;
+        const uint32_t sv = skv + (it_v % C::kStages) * kTileBytes;
+        const uint32_t sk = skv + (it_k % C::kStages) * kTileBytes;
+        const uint32_t ph = uint32_t(j) & 1u;
+        {
+          // keys behind the end of the run, inside its last tile: no row sees them, their V rows become zero
+          // (rows past s_kv already are: the TMA fill). The 128-byte swizzle permutes within a row only.
+          const int key = walk.base(j_lo + j);
+          const int from = walk.end(j_lo + j) - key, to = min(kBlockN, p.s_kv - key);
+          if (from < to) {
+            for (int c = 8 * from + lane; c < 8 * to; c += 32) {
+              st_shared_u4(sv + 16u * uint32_t(c), make_uint4(0, 0, 0, 0));
+              st_shared_u4(sv + kHalfBytes + 16u * uint32_t(c), make_uint4(0, 0, 0, 0));
+            }
+            fence_proxy_async();
+            __syncwarp();
+          }
+        }
+        for (int t = 0; t < kTiles; ++t) {
+          if (!(ok = wait_all(bar(C::kBarPSplit + t), ph, kStatusTimeoutP))) break;
+          tc_fence_after();
+          if (issuer) issue_pv_steps<0, 2 * kSplitChunks>(col_o(t), col_p(t), sv, j > 0);
+          __syncwarp();
+          if (!(ok = wait_all(bar(C::kBarPLast + t), ph, kStatusTimeoutP))) break;
+          tc_fence_after();
+          if (issuer) issue_pv_steps<2 * kSplitChunks, 8 - 2 * kSplitChunks>(col_o(t), col_p(t), sv, true);
+          __syncwarp();
+          if (!next) {
+            commit(C::kBarO + t);
+          } else {
+            if (t == 0 && !(ok = wait_full(it_k))) break;
+            if (issuer) issue_qk(tmem + 128u * t, sq + t * kTileBytes, sk);
+            __syncwarp();
+            commit(C::kBarS + t);
+          }
+        }
+      }
+      // every issued MMA must retire before TMEM is released
+      if (issuer) {
+        mma_commit(bar(C::kBarDrain));
+        drain_wait(bar(C::kBarDrain), 0, p.status);
+      }
+      __syncwarp();
+    }
+  } else {
+    regs_inc<C::kRegsSoftmax>();
+    // ------------------------------------------------------------ softmax + epilogue
+    const int t = (warp - 4) >> 2;
+    const int quad = warp & 3;
+    const uint32_t lane_off = uint32_t(quad * 32) << 16;
+    const uint32_t tS = tmem + lane_off + 128u * uint32_t(t);
+    const uint32_t tP = tS + 64u;
+    const uint32_t tO = tmem + lane_off + 128u * uint32_t(kTiles + t);
+    const float c = p.scale_log2;
+    const uint64_t c2 = f2_pack(c, c);
+    const int r_in = quad * 32 + lane;
+    const int row_pos = r_in / p.group;              // packed row -> query position in the tile, head in the group
+    const int row_head = r_in - row_pos * p.group;
+    const int it0 = i0 + t * p.tile_pos;             // the tile's first query
+    const int pos = p.q_start + it0 + row_pos;       // this row's key position
+    const int row_lo = pos - p.left, row_hi = min(pos + p.right, p.s_kv - 1);
+    const int row_ns = p.causal ? min(p.sinks, pos + 1) : p.sinks;
+    // what every row of the tile sees: keys below all_ns, keys of [all_lo, all_hi]
+    const int t_first = p.q_start + it0, t_last = t_first + p.tile_pos - 1;
+    const int all_lo = t_last - p.left, all_hi = min(t_first + p.right, p.s_kv - 1);
+    const int all_ns = p.causal ? min(p.sinks, t_first + 1) : p.sinks;
+    float m_run = -INFINITY;
+    uint64_t l_a = f2_pack(0.f, 0.f), l_b = f2_pack(0.f, 0.f);
+    bool ok = run;
+
+    for (int j = 0; ok && j < n_kv; ++j) {
+      ok = __all_sync(0xffffffffu, mbar_wait(bar(C::kBarS + t), uint32_t(j) & 1u, ctx, kStatusTimeoutS));
+      if (!ok) break;
+      if (t == kTiles - 1 && quad == 0 && lane == 0) mbar_arrive(bar(C::kBarRel + j % C::kRel));
+      tc_fence_after();
+      const int key = walk.base(j_lo + j);
+      const bool first_run = j_lo + j < walk.a_tiles;
+      const bool masked = !(key + kBlockN <= all_ns ||
+                            (!first_run && key >= all_lo && key + kBlockN - 1 <= all_hi));
+      uint32_t sa[64], sb[64];
+      tmem_ld64_wait(tS, sa);
+      tmem_ld64_nowait(tS + 64, sb);
+      float s[128];
+#pragma unroll
+      for (int i = 0; i < 64; ++i) s[i] = __uint_as_float(sa[i]);
+      const int ma = first_run ? 1 << 20 : row_lo - key, mb = row_hi - key, mn = row_ns - key;
+      if (masked) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const uint32_t bits = visible_bits(ma - 32 * w, mb - 32 * w, mn - 32 * w);
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!((bits >> i) & 1u)) s[32 * w + i] = -INFINITY;
+        }
+      }
+      float mx0 = fmax3(s[0], s[1], s[2]), mx1 = fmax3(s[3], s[4], s[5]);
+      float mx2 = fmax3(s[6], s[7], s[8]), mx3 = fmax3(s[9], s[10], s[11]);
+#pragma unroll
+      for (int i = 12; i < 60; i += 8) {
+        mx0 = fmax3(mx0, s[i], s[i + 1]);
+        mx1 = fmax3(mx1, s[i + 2], s[i + 3]);
+        mx2 = fmax3(mx2, s[i + 4], s[i + 5]);
+        mx3 = fmax3(mx3, s[i + 6], s[i + 7]);
+      }
+      mx0 = fmax3(mx0, s[60], s[61]);
+      mx1 = fmax3(mx1, s[62], s[63]);
+      tmem_ld64_wait_on(sb);
+#pragma unroll
+      for (int i = 0; i < 64; ++i) s[64 + i] = __uint_as_float(sb[i]);
+      if (masked) {
+#pragma unroll
+        for (int w = 2; w < 4; ++w) {
+          const uint32_t bits = visible_bits(ma - 32 * w, mb - 32 * w, mn - 32 * w);
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!((bits >> i) & 1u)) s[32 * w + i] = -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int i = 64; i < 120; i += 8) {
+        mx0 = fmax3(mx0, s[i], s[i + 1]);
+        mx1 = fmax3(mx1, s[i + 2], s[i + 3]);
+        mx2 = fmax3(mx2, s[i + 4], s[i + 5]);
+        mx3 = fmax3(mx3, s[i + 6], s[i + 7]);
+      }
+      mx0 = fmax3(mx0, s[120], s[121]);
+      mx1 = fmax3(mx1, s[122], s[123]);
+      mx2 = fmax3(mx2, s[124], s[125]);
+      mx3 = fmax3(mx3, s[126], s[127]);
+      const float m_new = fmaxf(m_run, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * c);
+      if (j == 0) {
+        m_run = m_new;
+      } else {
+        // rows whose running maximum grew by more than 2^8 (or from nothing) rescale O and l; O_t is quiescent
+        // here: S_t(j) ready implies every earlier P_t V has retired
+        const bool need = m_new > m_run + kRescaleThreshold;
+        if (__any_sync(0xffffffffu, need)) {
+          const float f = need ? ex2_approx(m_run - m_new) : 1.0f;
+          if (need) {
+            l_a = f2_fma(l_a, f2_pack(f, f), f2_pack(0.f, 0.f));
+            l_b = f2_fma(l_b, f2_pack(f, f), f2_pack(0.f, 0.f));
+            m_run = m_new;
+          }
+#pragma unroll 1
+          for (int c16 = 0; c16 < 8; ++c16) {
+            uint32_t o[16];
+            tmem_ld16_wait(tO + c16 * 16, o);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st16(tO + c16 * 16, o);
+          }
+          tmem_st_wait();
+        }
+      }
+      // exponentials in four 32-key chunks, each stored as bf16 P as soon as it is done. A row that has seen no
+      // key yet keeps m_run = -inf: its weights are exp2(-inf - 0) = 0.
+      const float m_use = m_run == -INFINITY ? 0.f : m_run;
+      const uint64_t nm2 = f2_pack(-m_use, -m_use);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int e = 32 * k + 2 * i;
+          float x0, x1;
+          f2_unpack(f2_fma(f2_pack(s[e], s[e + 1]), c2, nm2), x0, x1);
+          s[e] = ex2_approx(x0);
+          s[e + 1] = ex2_approx(x1);
+          pk[i] = pack_bf16x2(s[e], s[e + 1]);
+        }
+        tmem_st16(tP + 16 * k, pk);
+        if (k == kSplitChunks - 1) {
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(bar(C::kBarPSplit + t));
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(bar(C::kBarPLast + t));
+#pragma unroll
+      for (int i = 0; i < 128; i += 4) {
+        l_a = f2_add(l_a, f2_pack(s[i], s[i + 1]));
+        l_b = f2_add(l_b, f2_pack(s[i + 2], s[i + 3]));
+      }
+    }
+    float la0, la1, lb0, lb1;
+    f2_unpack(l_a, la0, la1);
+    f2_unpack(l_b, lb0, lb1);
+    const float l_run = (la0 + la1) + (lb0 + lb1);
+    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(C::kBarO + t), 0, ctx, kStatusTimeoutO));
+    // a CTA without keys writes its zeros too; an aborted one writes nothing
+    if (ok || (n_kv == 0 && *abort_flag == 0)) {
+      tc_fence_after();
+      const int i = it0 + row_pos;
+      const int head = kvh * p.group + row_head;
+      const bool valid = row_pos < p.tile_pos && i < p.s_q;
+      const bool none = n_kv == 0 || l_run == 0.f;
+      const float inv = 1.0f / l_run;
+      const long long ri = valid ? i : 0;
+      __nv_bfloat16* dst = p.o + (ri / p.o_rank_rows) * p.o_rank_stride + (long long)head * p.o_head_stride +
+                           (ri % p.o_rank_rows) * p.o_row_stride;
+      const long long part = ((long long)blockIdx.z * p.n_heads + head) * p.s_q + ri;
+#pragma unroll
+      for (int c4 = 0; c4 < 4; ++c4) {
+        uint32_t o[32];
+        tmem_ld32_wait(tO + c4 * 32, o);
+        if (!valid) continue;
+        if (p.part_o != nullptr) {
+          float4* d = reinterpret_cast<float4*>(p.part_o + part * 128 + c4 * 32);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            d[e] = none ? make_float4(0.f, 0.f, 0.f, 0.f)
+                        : make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
+                                      __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+        } else {
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            w[e] = none ? 0u : pack_bf16x2(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+          uint4* d = reinterpret_cast<uint4*>(dst + c4 * 32);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) d[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+        }
+      }
+      if (valid && p.part_ml != nullptr) {
+        reinterpret_cast<float2*>(p.part_ml)[part] = make_float2(m_run, none ? 0.f : l_run);
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kCols);
+  }
+}
+
+// One warp per output row: the splits' (O, m, l) joined in ascending order, normalised and rounded once.
+__global__ void __launch_bounds__(128) join_kernel(const Params p, int splits) {
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  const long long rows = (long long)p.n_heads * p.s_q;
+  if (row >= rows || *reinterpret_cast<volatile int*>(p.status) != 0) return;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
+  float m = -INFINITY;
+  for (int s = lane; s < splits; s += 32) m = fmaxf(m, ml[s * rows + row].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float m_use = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float2 v = ml[s * rows + row];
+    const float4 o = reinterpret_cast<const float4*>(p.part_o + (s * rows + row) * 128)[lane];
+    const float f = ex2_approx(v.x - m_use);
+    l += f * v.y;
+    acc.x += f * o.x;
+    acc.y += f * o.y;
+    acc.z += f * o.z;
+    acc.w += f * o.w;
+  }
+  const float inv = l == 0.f ? 0.f : 1.0f / l;
+  const long long i = row % p.s_q, head = row / p.s_q;
+  __nv_bfloat16* dst = p.o + (i / p.o_rank_rows) * p.o_rank_stride + head * p.o_head_stride +
+                       (i % p.o_rank_rows) * p.o_row_stride;
+  reinterpret_cast<uint2*>(dst)[lane] =
+      make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+}
+
+// ---------------------------------------------------------------- host
+constexpr int64_t kMaxPos = 1ll << 29;  // positions, window sides and lengths stay inside int32 sums
+constexpr int kMaxSplits = 64;
+
+struct Shape {
+  int64_t n_heads, n_kv_heads, s_q, s_kv, left, right, sinks, q_start;
+  int32_t causal;
+};
+
+static int check_shape(const Shape& s) {
+  if (s.n_heads < 1 || s.n_kv_heads < 1 || s.n_heads > 65535 || s.n_heads % s.n_kv_heads ||
+      s.n_heads / s.n_kv_heads > 128 || s.s_q < 1 || s.s_kv < 1 || s.s_q > kMaxPos || s.s_kv > kMaxPos ||
+      s.sinks < 0 || s.q_start < -kMaxPos || s.q_start > kMaxPos)
+    return H3_ERR_SHAPE;
+  return H3_OK;
+}
+
+// The launch shape of a call.
+struct Plan {
+  int tiles;    // Q tiles per CTA
+  int tile_pos; // query positions per Q tile
+  unsigned grid_x;
+  int splits;
+};
+
+// Q tiles per CTA: two (256 packed rows, one CTA an SM) where the rows fill them, else one (two CTAs an SM).
+// Splits: only when the unsplit grid leaves CTA slots empty; then as many as fill them, with at least two
+// key tiles each.
+static int make_plan(const Shape& s, int64_t splits_asked, Plan& pl) {
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return H3_ERR_CUDA;
+  const int group = (int)(s.n_heads / s.n_kv_heads);
+  pl.tile_pos = 128 / group;
+  pl.tiles = s.s_q <= pl.tile_pos ? 1 : 2;
+  const int64_t per_cta = (int64_t)pl.tiles * pl.tile_pos;
+  pl.grid_x = (unsigned)((s.s_q + per_cta - 1) / per_cta);
+  const int64_t ctas = (int64_t)pl.grid_x * s.n_kv_heads, slots = (int64_t)sms * (pl.tiles == 1 ? 2 : 1);
+  const int64_t left = s.left < 0 || s.left > kMaxPos ? kMaxPos : s.left;
+  const int64_t right = s.causal ? 0 : (s.right < 0 || s.right > kMaxPos ? kMaxPos : s.right);
+  const int64_t span = std::min(s.s_kv, left + right + per_cta) + std::min(s.sinks, s.s_kv);
+  const int64_t tiles = (std::min(span, s.s_kv) + kBlockN - 1) / kBlockN;
+  int64_t splits = splits_asked;
+  if (splits == 0) splits = std::min(slots / std::max<int64_t>(ctas, 1), tiles / 2);
+  pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits));
+  return H3_OK;
+}
+
+static int64_t workspace_bytes(const Shape& s, const Plan& pl) {
+  return pl.splits == 1 ? 0 : (int64_t)pl.splits * s.n_heads * s.s_q * (128 + 2) * (int64_t)sizeof(float);
+}
+
+// [kv_heads][s_q][group][128] view of q: box 64 x group x tile_pos x 1, SW128, zero fill.
+static int make_q_map(CUtensorMap* map, const void* q, const Shape& s, int64_t head_stride, int64_t row_stride,
+                      int tile_pos) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (!enc) return H3_ERR_DRIVER;
+  const cuuint64_t group = (cuuint64_t)(s.n_heads / s.n_kv_heads);
+  const cuuint64_t hs = (cuuint64_t)(s.n_heads > 1 ? head_stride : s.s_q * row_stride);
+  cuuint64_t dims[4] = {128, group, (cuuint64_t)s.s_q, (cuuint64_t)s.n_kv_heads};
+  cuuint64_t strides[3] = {hs * 2, (cuuint64_t)row_stride * 2, hs * group * 2};
+  cuuint32_t box[4] = {64, (cuuint32_t)group, (cuuint32_t)tile_pos, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(q), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? H3_OK : H3_ERR_TENSOR_MAP;
+}
+
+template <int kTiles>
+static int launch(cudaStream_t st, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const Params& p,
+                  const Plan& pl, unsigned kv_heads) {
+  using C = Cfg<kTiles>;
+  auto* kern = window_kernel<kTiles>;
+  // setmaxnreg draws on the registers the CTA is launched with: the split must fit them
+  static const int regs = [&] {
+    cudaFuncAttributes a;
+    return cudaFuncGetAttributes(&a, kern) == cudaSuccess ? a.numRegs : 0;
+  }();
+  if (regs * C::kThreads < 128 * C::kRegsControl + 128 * kTiles * C::kRegsSoftmax) return H3_ERR_UNSUPPORTED;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem) != cudaSuccess)
+    return H3_ERR_LAUNCH;
+  kern<<<dim3(pl.grid_x, kv_heads, (unsigned)pl.splits), C::kThreads, C::kSmem, st>>>(q, k, v, p);
+  return cudaGetLastError() == cudaSuccess ? H3_OK : H3_ERR_LAUNCH;
+}
+
+}  // namespace window
+}  // namespace h3
+
+using namespace h3;
+using namespace h3::window;
+
+extern "C" int h3_window_attn_plan(int64_t n_heads, int64_t n_kv_heads, int64_t s_q, int64_t s_kv, int64_t left,
+                                   int64_t right, int64_t sinks, int32_t causal, int64_t q_start, int64_t splits,
+                                   int64_t* ws_bytes) {
+  if (!ws_bytes) return H3_ERR_NULL;
+  const Shape s = {n_heads, n_kv_heads, s_q, s_kv, left, right, sinks, q_start, causal};
+  int rc;
+  if ((rc = check_shape(s)) != H3_OK) return rc;
+  if (splits < 0 || splits > kMaxSplits) return H3_ERR_SHAPE;
+  Plan pl;
+  if ((rc = make_plan(s, splits, pl)) != H3_OK) return rc;
+  *ws_bytes = workspace_bytes(s, pl);
+  return pl.splits;
+}
+
+extern "C" int h3_window_attn(const void* q, const void* k, const void* v, void* o, int64_t n_heads,
+                              int64_t n_kv_heads, int64_t s_q, int64_t s_kv, int64_t q_head_stride,
+                              int64_t q_row_stride, int64_t kv_head_stride, int64_t kv_row_stride, int64_t o_rank_rows,
+                              int64_t o_rank_stride, int64_t o_head_stride, int64_t o_row_stride, float softmax_scale,
+                              int64_t left, int64_t right, int64_t sinks, int32_t causal, int64_t q_start,
+                              int64_t splits, void* workspace, int64_t ws_bytes, int32_t* status, void* stream) {
+  if (!q || !k || !v || !o || !status) return H3_ERR_NULL;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || (workspace && !aligned16(workspace)) ||
+      (reinterpret_cast<uintptr_t>(status) & 3u))
+    return H3_ERR_ALIGN;
+  const Shape s = {n_heads, n_kv_heads, s_q, s_kv, left, right, sinks, q_start, causal};
+  int rc;
+  if ((rc = check_shape(s)) != H3_OK) return rc;
+  if (o_rank_rows < 1 || splits < 1 || splits > kMaxSplits) return H3_ERR_SHAPE;
+  if (!(softmax_scale > 0.f) || !std::isfinite(softmax_scale)) return H3_ERR_SHAPE;
+  if (q_row_stride < 128 || kv_row_stride < 128 || o_row_stride < 128 || (q_row_stride % 8) || (kv_row_stride % 8) ||
+      (q_head_stride % 8) || (kv_head_stride % 8) || (o_row_stride % 8) || (o_head_stride % 8) ||
+      (o_rank_stride % 8) || q_head_stride < 0 || kv_head_stride < 0 || o_head_stride < 0 || o_rank_stride < 0 ||
+      (n_heads > 1 && q_head_stride == 0) || (n_kv_heads > 1 && kv_head_stride == 0))
+    return H3_ERR_STRIDE;
+  Plan pl;
+  if ((rc = make_plan(s, splits, pl)) != H3_OK) return rc;
+  if (pl.splits > 1 && !workspace) return H3_ERR_NULL;
+  if (ws_bytes < workspace_bytes(s, pl)) return H3_ERR_WORKSPACE;
+
+  CUtensorMap mq, mk, mv;
+  const long long kvhs = n_kv_heads > 1 ? kv_head_stride : s_kv * kv_row_stride;
+  if ((rc = make_q_map(&mq, q, s, q_head_stride, q_row_stride, pl.tile_pos)) != H3_OK) return rc;
+  if ((rc = make_head_map(&mk, k, s_kv, n_kv_heads, kv_row_stride, kvhs)) != H3_OK) return rc;
+  if ((rc = make_head_map(&mv, v, s_kv, n_kv_heads, kv_row_stride, kvhs)) != H3_OK) return rc;
+
+  Params p;
+  p.n_heads = (int)n_heads;
+  p.group = (int)(n_heads / n_kv_heads);
+  p.s_q = (int)s_q;
+  p.s_kv = (int)s_kv;
+  p.left = (int)(left < 0 || left > kMaxPos ? kMaxPos : left);
+  p.right = causal ? 0 : (int)(right < 0 || right > kMaxPos ? kMaxPos : right);
+  p.sinks = (int)std::min(sinks, s_kv);
+  p.causal = causal ? 1 : 0;
+  p.q_start = (int)q_start;
+  p.tile_pos = pl.tile_pos;
+  p.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
+  p.o = reinterpret_cast<__nv_bfloat16*>(o);
+  p.o_rank_rows = o_rank_rows;
+  p.o_rank_stride = o_rank_stride;
+  p.o_head_stride = o_head_stride;
+  p.o_row_stride = o_row_stride;
+  p.part_o = pl.splits > 1 ? reinterpret_cast<float*>(workspace) : nullptr;
+  p.part_ml = pl.splits > 1 ? p.part_o + (int64_t)pl.splits * n_heads * s_q * 128 : nullptr;
+  p.status = status;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  rc = pl.tiles == 2 ? launch<2>(st, mq, mk, mv, p, pl, (unsigned)n_kv_heads)
+                     : launch<1>(st, mq, mk, mv, p, pl, (unsigned)n_kv_heads);
+  if (rc != H3_OK || pl.splits == 1) return rc;
+  join_kernel<<<(unsigned)((n_heads * s_q + 3) / 4), 128, 0, st>>>(p, pl.splits);
+  return cudaGetLastError() == cudaSuccess ? H3_OK : H3_ERR_LAUNCH;
+}

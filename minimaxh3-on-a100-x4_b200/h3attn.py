@@ -12,11 +12,13 @@ Reference counterparts:
   head_to_seq_unpack   transpose/reshape ahead of out_proj, sp_runtime.py:125
 Without a counterpart in the reference:
   RopePositions, rope_axes   rotary positions over several axes (time, height, width)
+  window_attention           sliding window with first tokens that stay visible
 """
 from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import math
 import os
 
@@ -38,6 +40,7 @@ _ERRORS = {
     -9: "a CUDA runtime call failed",
     -10: "the call needs more than the no-alloc entry point's static scratch",
     -11: "a kernel gave up waiting (bounded-wait timeout)",
+    -12: "the workspace is smaller than the call needs",
 }
 STATUS_NAMES = {
     0: "ok", 1: "timeout waiting for Q tiles", 2: "timeout in the K/V ring", 3: "timeout waiting for S",
@@ -93,6 +96,11 @@ def lib() -> ctypes.CDLL:
         L.h3_qknorm_rope_pack_peer.restype = ctypes.c_int
         L.h3_attn_fwd_peer.argtypes = [vp] * 5 + [i64] * 11 + [ctypes.c_float, i32p, vp]
         L.h3_attn_fwd_peer.restype = ctypes.c_int
+        L.h3_window_attn_plan.argtypes = [i64] * 7 + [ctypes.c_int32, i64, i64, vp]
+        L.h3_window_attn_plan.restype = ctypes.c_int
+        L.h3_window_attn.argtypes = [vp] * 4 + [i64] * 12 + [f32, i64, i64, i64, ctypes.c_int32, i64, i64, vp, i64, i32p,
+                                     vp]
+        L.h3_window_attn.restype = ctypes.c_int
         L.h3_rope_axes.argtypes = [vp, i64, i64, vp, ctypes.c_int32, i64, vp, vp, ctypes.c_int32, vp, i64, i64, i64,
                                    i64, vp]
         L.h3_rope_axes.restype = ctypes.c_int
@@ -161,6 +169,20 @@ def check_status(device=None) -> None:
 
 
 # ----------------------------------------------------------------------------- attention
+def _out_layout(layout: str, H: int, sq: int, world: int):
+    """(shape, rows per rank, rank / head / row strides) of an attention output layout."""
+    if layout == "head":
+        return (H, sq, D), sq, 0, sq * D, D
+    if layout == "token":
+        return (sq, H * D), sq, 0, D, H * D
+    if layout == "send":
+        if sq % world:
+            raise H3Error(f"send layout needs rows {sq} divisible by world {world}")
+        sl = sq // world
+        return (world, H, sl, D), sl, H * sl * D, sl * D, D
+    raise H3Error(f"unknown layout {layout!r}")
+
+
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, s_kv: int | None = None,
               scale: float | None = None, out: torch.Tensor | None = None, layout: str = "head",
               world: int = 1, variant: int | None = None) -> torch.Tensor:
@@ -185,17 +207,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, s_kv: int | Non
     if not 1 <= s_kv <= skv_alloc:
         raise H3Error(f"s_kv={s_kv} outside [1, {skv_alloc}]")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if layout == "head":
-        shape, rank_rows, rank_stride, head_stride, row_stride = (H, sq, D), sq, 0, sq * D, D
-    elif layout == "token":
-        shape, rank_rows, rank_stride, head_stride, row_stride = (sq, H * D), sq, 0, D, H * D
-    elif layout == "send":
-        if sq % world:
-            raise H3Error(f"send layout needs rows {sq} divisible by world {world}")
-        sl = sq // world
-        shape, rank_rows, rank_stride, head_stride, row_stride = (world, H, sl, D), sl, H * sl * D, sl * D, D
-    else:
-        raise H3Error(f"unknown layout {layout!r}")
+    shape, rank_rows, rank_stride, head_stride, row_stride = _out_layout(layout, H, sq, world)
     if out is None:
         out = torch.empty(shape, dtype=torch.bfloat16, device=q.device)
     else:
@@ -210,6 +222,75 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, s_kv: int | Non
     else:
         rc = lib().h3_attn_fwd_variant(*args, int(variant), _stream())
     _check(rc, "h3_attn_fwd")
+    return out
+
+
+# ----------------------------------------------------------------------------- windowed attention
+@functools.lru_cache(maxsize=4096)
+def _window_plan(dev_index: int, *shape) -> tuple:
+    """(splits, workspace bytes) of a windowed attention call on the current device; a pure function of
+    its sizes."""
+    n = ctypes.c_int64()
+    rc = lib().h3_window_attn_plan(*shape, ctypes.byref(n))
+    if rc < 0:
+        _check(rc, "h3_window_attn_plan")
+    return rc, n.value
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: int | None, right: int | None,
+                     sinks: int = 0, causal: bool = False, q_start: int | None = None, s_kv: int | None = None,
+                     scale: float | None = None, out: torch.Tensor | None = None, layout: str = "head",
+                     world: int = 1, splits: int | None = None) -> torch.Tensor:
+    """Attention with a sliding window and first tokens that stay visible: q [H, Sq, 128], k/v [Hkv, Skv, 128]
+    (bf16, last dim contiguous, strides multiples of 8; H a multiple of Hkv, query head h reads key head
+    h // (H // Hkv)). Query i sits at key position p = q_start + i and sees key j < s_kv when j < sinks or
+    p - left <= j <= p + right; causal=True also asks j <= p. None for left / right: no bound on that side. q_start
+    defaults to max(s_kv - Sq, 0): the queries are the last keys. A query that sees no key gets zeros. K and V
+    may hold anything at keys that no query sees. out / layout / world as attention().
+    splits: how many parts the key axis is worked in (None: chosen by the call's sizes); with 1 a query row's
+    bits do not depend on how many heads share the call."""
+    for n, t in (("q", q), ("k", k), ("v", v)):
+        _cuda(t, n)
+        if t.dim() != 3 or t.shape[-1] != D or t.stride(-1) != 1:
+            raise H3Error(f"{n} must be [heads, rows, 128] with a contiguous last dim, got {tuple(t.shape)}")
+    dev = q.device
+    _together(dev, k=k, v=v, out=out)
+    H, sq, _ = q.shape
+    hk, skv_alloc, _ = k.shape
+    if v.shape != k.shape or hk < 1 or H % hk:
+        raise H3Error("k and v must share a shape, and the query heads be a multiple of the key heads")
+    q_st, k_st, v_st = (tuple(t.stride(i) if t.shape[i] > 1 else D for i in (0, 1)) for t in (q, k, v))
+    if k_st != v_st:
+        raise H3Error("k and v must share strides")
+    s_kv = skv_alloc if s_kv is None else int(s_kv)
+    if not 1 <= s_kv <= skv_alloc:
+        raise H3Error(f"s_kv={s_kv} outside [1, {skv_alloc}]")
+    for n, side in (("left", left), ("right", right)):
+        if side is not None and side < 0:
+            raise H3Error(f"{n}={side}: a window side is a count of keys, or None for no bound")
+    if sinks < 0 or (splits is not None and splits < 1):
+        raise H3Error(f"sinks={sinks}, splits={splits} out of range")
+    q_start = max(s_kv - sq, 0) if q_start is None else int(q_start)
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    shape, rank_rows, rank_stride, head_stride, row_stride = _out_layout(layout, H, sq, world)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+    else:
+        _cuda(out, "out")
+        if tuple(out.shape) != tuple(shape) or not out.is_contiguous():
+            raise H3Error(f"out must be contiguous {shape}, got {tuple(out.shape)}")
+    # sides past every key are no bound: keep them inside the C call's integers
+    big = sq + s_kv + abs(q_start)
+    lo, hi = (-1 if side is None or side > big else int(side) for side in (left, right))
+    sinks = min(int(sinks), s_kv)
+    with _on(dev):
+        n_splits, ws_bytes = _window_plan(dev.index, H, hk, sq, s_kv, lo, hi, sinks, int(causal), q_start, splits or 0)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+        rc = lib().h3_window_attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), H, hk, sq, s_kv,
+                                  *q_st, *k_st, rank_rows, rank_stride,
+                                  head_stride, row_stride, scale, lo, hi, sinks, int(causal), q_start, n_splits,
+                                  ws.data_ptr() if ws_bytes else None, ws_bytes, status_word(dev).data_ptr(), _stream())
+    _check(rc, "h3_window_attn")
     return out
 
 

@@ -62,3 +62,65 @@ def test_rope_has_no_cpu_path():
     rp = O.RopePositions(torch.zeros(4, 1, dtype=torch.int32), f, a)
     with pytest.raises(O.H3Error):
         O.rope_axes(torch.zeros(4, 1, 128, dtype=torch.bfloat16), rp)
+
+
+def test_window_rejects_bad_arguments_before_launch(L):
+    p, st = ctypes.c_void_p(0x1000), ctypes.c_void_p(0x2000)
+    #     q  k  v  o  H  Hk sq  skv  q strides    kv strides   rows rank head     row  scale
+    ok = [p, p, p, p, 8, 2, 64, 500, 64 * 128, 128, 500 * 128, 128, 64, 0, 64 * 128, 128, ctypes.c_float(0.09),
+          100, 0, 4, 1, 436, 1, None, 0, st, None]  # left right sinks causal q_start splits ws bytes status stream
+    for at, value, code in ((0, None, -1), (25, None, -1), (3, ctypes.c_void_p(0x1008), -2), (4, 9, -3), (5, 0, -3),
+                            (6, 0, -3), (7, 0, -3), (7, (1 << 29) + 1, -3), (19, -1, -3), (21, 1 << 30, -3),
+                            (22, 0, -3), (22, 65, -3), (12, 0, -3), (16, ctypes.c_float(0.0), -3),
+                            (16, ctypes.c_float(float("nan")), -3), (9, 100, -4), (9, 120, -4), (11, 64, -4),
+                            (8, 0, -4), (10, 0, -4), (15, 64, -4), (14, -8, -4)):
+        bad = list(ok)
+        bad[at] = value
+        assert L.h3_window_attn(*bad) == code, (at, value)
+    bad = list(ok)
+    bad[4], bad[5] = 258, 2  # more than 128 query heads to a key head
+    assert L.h3_window_attn(*bad) == -3
+    assert L.h3_window_attn_plan(8, 2, 64, 500, 100, 0, 4, 1, 436, 0, None) == -1
+    n = ctypes.c_int64()
+    assert L.h3_window_attn_plan(8, 3, 64, 500, 100, 0, 4, 1, 436, 0, ctypes.byref(n)) == -3
+    assert L.h3_window_attn_plan(8, 2, 64, 500, 100, 0, 4, 1, 436, 65, ctypes.byref(n)) == -3
+
+
+def _walk(left, right, sinks, causal, s_kv, p_first, p_last, tile=128):
+    """The key tiles of a CTA whose rows sit at positions p_first .. p_last: (first key, end of its run)."""
+    lo, hi = max(0, p_first - left), min(s_kv - 1, p_last + right)
+    ns = max(0, min(sinks, p_last + 1)) if causal else sinks
+    window = lo <= hi
+    joined = window and lo <= ns
+    out = [] if joined else [(b, ns) for b in range(0, ns, tile)]
+    if window:
+        start, end = (0, max(hi + 1, ns)) if joined else (lo, hi + 1)
+        out += [(b, end) for b in range(start, end, tile)]
+    return out
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("left,right,sinks", [(0, 0, 0), (5, 3, 0), (5, 0, 7), (200, 40, 150), (1000, 1000, 300)])
+def test_window_walk_covers_each_visible_key_once(left, right, sinks, causal):
+    """The walk the kernel takes, restated: every key that a row sees lies in exactly one tile in which the row's mask
+    lets it through, tiles start inside the keys, and no key of a run is one that no row sees."""
+    s_kv, right = 700, 0 if causal else right
+    for p_first, p_last in ((0, 0), (0, 255), (100, 227), (600, 699), (690, 800), (-40, 20), (-300, -100), (900, 950)):
+        tiles = _walk(left, right, min(sinks, s_kv), causal, s_kv, p_first, p_last)
+        ns_all = max(0, min(sinks, p_last + 1)) if causal else sinks
+        first_run = [t for t in tiles if t[1] == ns_all and t[0] % 128 == 0 and t[0] < ns_all]
+        assert all(0 <= b < s_kv for b, _ in tiles)
+        seen_any = set()
+        for p in {p_first, (p_first + p_last) // 2, p_last}:
+            see = {j for j in range(s_kv) if (j < sinks or p - left <= j <= p + right) and (not causal or j <= p)}
+            seen_any |= see
+            got = []
+            for b, end in tiles:
+                separate = (b, end) in first_run and len(tiles) > 0 and end == ns_all and max(0, p_first - left) > ns_all
+                for j in range(b, min(b + 128, s_kv)):
+                    ns = min(sinks, p + 1) if causal else sinks
+                    in_window = (not separate) and max(0, p - left) <= j <= min(s_kv - 1, p + right)
+                    if in_window or j < ns:
+                        assert j < end
+                        got.append(j)
+            assert sorted(got) == sorted(see), (p_first, p_last, p)
