@@ -235,6 +235,26 @@ int h3_gemm_bf16(const void* a, int64_t m, int64_t a_chunks, int64_t a_chunk_col
                  int64_t a_row_stride, const void* w, int64_t n_out, int64_t w_row_stride, void* c,
                  int64_t c_row_stride, int32_t epilogue, int32_t* status, void* stream);
 
+/* The projection GEMM with low-rank adapters of many requests. No counterpart in the reference.
+ *   c[t] = epilogue( W a[t] + scale[g] * B_g (A_g a[t]) ),   g = row_adapter[t]; outside [0, n_adapters): W a[t] alone
+ * a, w, c, epilogue as h3_gemm_bf16 (epilogue 1 with its roundings). The adapters are stacked: lora_a
+ * [n_adapters * rank][k] (rows of adapter g from g * rank), lora_b [n rows of w][n_adapters * rank] (columns of
+ * adapter g from g * rank), bf16, row strides multiples of 8; rank 8, 16, 32 or a multiple of 64 up to 256 (a smaller
+ * one is padded with zeros), n_adapters * rank <= 65536; scale fp32 [n_adapters], row_adapter int32 [m]. fp32
+ * accumulation; A_g a[t] is rounded to bf16 (after the scale) when m > 64 and kept in fp32 below. The bits of an
+ * output row do not depend on the other rows, for calls of m <= 64 and of m > 64 each. Above 64 rows, lora_b must be
+ * finite where a row of the same 256-row block uses its 64 stacked columns.
+ * h3_gemm_adapters_workspace returns the bytes of 16-byte aligned workspace that the call needs (or an error); it may
+ * be reused once the call's work on the stream is done. */
+int64_t h3_gemm_adapters_workspace(int64_t m, int64_t a_chunks, int64_t a_chunk_cols, int64_t n_out, int32_t epilogue,
+                                   int64_t rank, int64_t n_adapters);
+int h3_gemm_adapters(const void* a, int64_t m, int64_t a_chunks, int64_t a_chunk_cols, int64_t a_chunk_stride,
+                     int64_t a_row_stride, const void* w, int64_t n_out, int64_t w_row_stride, const void* lora_a,
+                     int64_t lora_a_row_stride, const void* lora_b, int64_t lora_b_row_stride, int64_t rank,
+                     int64_t n_adapters, const float* scale, const int32_t* row_adapter, void* c,
+                     int64_t c_row_stride, int32_t epilogue, void* workspace, int64_t ws_bytes, int32_t* status,
+                     void* stream);
+
 /* AdaLN modulation of the DiT block (the host model's norm + _mod_scale_shift, harness/sp_runtime.py:
  * 209-210 and :214-215), optionally after its gated residual (_mod_gate, :212-213), in one pass:
  *   xr = x + gate[seg] * y   (when y != NULL and the token is in a segment; else xr = x), stored to

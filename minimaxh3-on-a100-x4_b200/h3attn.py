@@ -13,6 +13,7 @@ Reference counterparts:
 Without a counterpart in the reference:
   RopePositions, rope_axes   rotary positions over several axes (time, height, width)
   window_attention           sliding window with first tokens that stay visible
+  linear_lora                low-rank adapters of many requests beside a shared projection
 """
 from __future__ import annotations
 
@@ -86,6 +87,11 @@ def lib() -> ctypes.CDLL:
             getattr(L, name).restype = ctypes.c_int
         L.h3_gemm_bf16.argtypes = [vp, i64, i64, i64, i64, i64, vp, i64, i64, vp, i64, ctypes.c_int32, i32p, vp]
         L.h3_gemm_bf16.restype = ctypes.c_int
+        L.h3_gemm_adapters_workspace.argtypes = [i64, i64, i64, i64, ctypes.c_int32, i64, i64]
+        L.h3_gemm_adapters_workspace.restype = i64
+        L.h3_gemm_adapters.argtypes = [vp, i64, i64, i64, i64, i64, vp, i64, i64, vp, i64, vp, i64, i64, i64, vp, vp, vp,
+                                       i64, ctypes.c_int32, vp, i64, i32p, vp]
+        L.h3_gemm_adapters.restype = ctypes.c_int
         L.h3_norm_modulate.argtypes = [vp, i64, vp, i64, vp, vp, i64, vp, vp, i64, vp, vp, i64, i64, i64,
                                        ctypes.c_float, vp]
         L.h3_norm_modulate.restype = ctypes.c_int
@@ -544,13 +550,9 @@ def head_to_seq_unpack(recv: torch.Tensor, out: torch.Tensor | None = None) -> t
 
 
 # ----------------------------------------------------------------------------- projection GEMM
-def linear(a: torch.Tensor, weight: torch.Tensor, out: torch.Tensor | None = None,
-           epilogue: str = "none") -> torch.Tensor:
-    """Row-independent a @ weight.T (bf16, fp32 accumulate): the bits of an output row depend only
-    on that row of `a`, never on how many rows the call has.
-      a: [m, k] with a contiguous last dim, or head-major [H, m, 128] (read in place as [m, H*128]);
-      weight: [n, k] (nn.Linear layout); epilogue "swiglu": weight = [gate; up] (2F rows) and the
-      result is silu(a @ gate.T) * (a @ up.T), [m, F]."""
+def _linear_args(a, weight, out, epilogue):
+    """Checks shared by the projections; returns (m, chunks, chunk columns, chunk stride, row stride, output columns,
+    epilogue code, out)."""
     _cuda(a, "a")
     _cuda(weight, "weight")
     if weight.dim() != 2 or weight.stride(-1) != 1:
@@ -582,10 +584,97 @@ def linear(a: torch.Tensor, weight: torch.Tensor, out: torch.Tensor | None = Non
         _cuda(out, "out")
         if tuple(out.shape) != (m, n) or out.stride(-1) != 1:
             raise H3Error(f"out must be [{m}, {n}] with a contiguous last dim")
+    return m, chunks, chunk_cols, chunk_stride, row_stride, n, ep, out
+
+
+def linear(a: torch.Tensor, weight: torch.Tensor, out: torch.Tensor | None = None,
+           epilogue: str = "none") -> torch.Tensor:
+    """Row-independent a @ weight.T (bf16, fp32 accumulate): the bits of an output row depend only
+    on that row of `a`, never on how many rows the call has.
+      a: [m, k] with a contiguous last dim, or head-major [H, m, 128] (read in place as [m, H*128]);
+      weight: [n, k] (nn.Linear layout); epilogue "swiglu": weight = [gate; up] (2F rows) and the
+      result is silu(a @ gate.T) * (a @ up.T), [m, F]."""
+    m, chunks, chunk_cols, chunk_stride, row_stride, n, ep, out = _linear_args(a, weight, out, epilogue)
     rc = lib().h3_gemm_bf16(a.data_ptr(), m, chunks, chunk_cols, chunk_stride, row_stride, weight.data_ptr(), n,
                             weight.stride(0), out.data_ptr(), out.stride(0), ep, status_word(a.device).data_ptr(),
                             _stream())
     _check(rc, "h3_gemm_bf16")
+    return out
+
+
+# ----------------------------------------------------------------------------- adapters beside a projection
+_RANKS = (8, 16, 32, 64, 128, 192, 256)
+
+
+def stack_adapters(pairs, scales, device=None):
+    """(lora_a, lora_b, scale) as linear_lora takes them, from [(A [r, k], B [n, r]), ...] with ranks up to 256 and one
+    factor each: ranks are padded with zeros to the smallest of 8, 16, 32, 64, 128, 192, 256 that holds them all. Laid
+    out once per set of adapters."""
+    pairs = list(pairs)
+    if not pairs or len(scales) != len(pairs):
+        raise H3Error("one (A, B) pair and one scale per adapter")
+    k, n = pairs[0][0].shape[1], pairs[0][1].shape[0]
+    for A, B in pairs:
+        if A.dim() != 2 or B.dim() != 2 or A.shape[1] != k or B.shape[0] != n or A.shape[0] != B.shape[1]:
+            raise H3Error("adapters must be A [r, k], B [n, r] with one k and one n")
+    most = max(A.shape[0] for A, _ in pairs)
+    rank = next((r for r in _RANKS if r >= most), None)
+    if rank is None:
+        raise H3Error(f"rank {most} is above {_RANKS[-1]}")
+    device = pairs[0][0].device if device is None else device
+    lora_a = torch.zeros(len(pairs) * rank, k, dtype=torch.bfloat16, device=device)
+    lora_b = torch.zeros(n, len(pairs) * rank, dtype=torch.bfloat16, device=device)
+    for i, (A, B) in enumerate(pairs):
+        lora_a[i * rank:i * rank + A.shape[0]] = A
+        lora_b[:, i * rank:i * rank + A.shape[0]] = B
+    return lora_a, lora_b, torch.tensor([float(x) for x in scales], dtype=torch.float32, device=device)
+
+
+@functools.lru_cache(maxsize=4096)
+def _adapters_workspace(dev_index: int, *shape) -> int:
+    """Workspace bytes of a call of these sizes on the current device."""
+    n = lib().h3_gemm_adapters_workspace(*shape)
+    if n < 0:
+        _check(n, "h3_gemm_adapters_workspace")
+    return n
+
+
+def linear_lora(a: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
+                scale: torch.Tensor, rows: torch.Tensor, out: torch.Tensor | None = None,
+                epilogue: str = "none") -> torch.Tensor:
+    """linear() with a low-rank adapter per row: a @ weight.T + scale[g] * (a @ A_g.T) @ B_g.T with g = rows[row]
+    (outside [0, adapters): the projection alone), rounded once; epilogue "swiglu" as linear().
+      a, weight, out: as linear(); lora_a: [adapters * rank, k], lora_b: [weight rows, adapters * rank] bf16, adapter g at
+      [g * rank, (g + 1) * rank) of both (stack_adapters lays them out); rank 8, 16, 32 or a multiple of 64 up to 256;
+      scale: fp32 [adapters]; rows: int32 [m] (segment_rows makes it from token segments).
+    A row's bits do not depend on the other rows among calls of up to 64 rows, and among longer ones. In calls of more
+    than 64 rows B must be finite: rows of a 256-row block meet each other's adapters with zero weights."""
+    m, chunks, chunk_cols, chunk_stride, row_stride, n, ep, out = _linear_args(a, weight, out, epilogue)
+    _cuda(lora_a, "lora_a")
+    _cuda(lora_b, "lora_b")
+    _cuda(scale, "scale", torch.float32)
+    _cuda(rows, "rows", torch.int32)
+    dev = a.device
+    _together(dev, weight=weight, lora_a=lora_a, lora_b=lora_b, scale=scale, rows=rows, out=out)
+    if scale.dim() != 1 or scale.shape[0] < 1 or not scale.is_contiguous():
+        raise H3Error("scale must be a contiguous fp32 [adapters]")
+    n_adapters = scale.shape[0]
+    if lora_a.dim() != 2 or lora_a.shape[1] != weight.shape[1] or lora_a.shape[0] % n_adapters or lora_a.stride(1) != 1:
+        raise H3Error(f"lora_a must be [{n_adapters} * rank, {weight.shape[1]}] with a contiguous last dim")
+    if tuple(lora_b.shape) != (weight.shape[0], lora_a.shape[0]) or lora_b.stride(1) != 1:
+        raise H3Error(f"lora_b must be [{weight.shape[0]}, {lora_a.shape[0]}] with a contiguous last dim")
+    if tuple(rows.shape) != (m,) or not rows.is_contiguous():
+        raise H3Error(f"rows must be a contiguous int32 [{m}]")
+    rank = lora_a.shape[0] // n_adapters
+    with _on(dev):
+        ws_bytes = _adapters_workspace(dev.index, m, chunks, chunk_cols, n, ep, rank, n_adapters)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        rc = lib().h3_gemm_adapters(a.data_ptr(), m, chunks, chunk_cols, chunk_stride, row_stride, weight.data_ptr(), n,
+                                    weight.stride(0), lora_a.data_ptr(), lora_a.stride(0), lora_b.data_ptr(),
+                                    lora_b.stride(0), rank, n_adapters, scale.data_ptr(), rows.data_ptr(),
+                                    out.data_ptr(), out.stride(0), ep, ws.data_ptr(), ws_bytes,
+                                    status_word(dev).data_ptr(), _stream())
+    _check(rc, "h3_gemm_adapters")
     return out
 
 

@@ -124,3 +124,60 @@ def test_window_walk_covers_each_visible_key_once(left, right, sinks, causal):
                         assert j < end
                         got.append(j)
             assert sorted(got) == sorted(see), (p_first, p_last, p)
+
+
+def test_adapters_reject_bad_arguments_before_launch(L):
+    p, st = ctypes.c_void_p(0x1000), ctypes.c_void_p(0x2000)
+    #     a  m  chunks cols cstride row  w  n    wrow A  Arow B  Brow rank na scale rows c  crow ep ws bytes status stream
+    ok = [p, 300, 1, 512, 0, 512, p, 256, 512, p, 512, p, 64, 16, 4, p, p, p, 256, 0, p, 0, st, None]
+    for at, value, code in ((0, None, -1), (9, None, -1), (11, None, -1), (15, None, -1), (16, None, -1), (20, None, -1),
+                            (9, ctypes.c_void_p(0x1008), -2), (20, ctypes.c_void_p(0x1008), -2),
+                            (16, ctypes.c_void_p(0x1002), -2), (13, 12, -3), (13, 4, -3), (13, 96, -3), (13, 320, -3),
+                            (14, 0, -3), (14, 4097, -3), (7, 100, -3), (19, 2, -3), (10, 504, -4), (12, 56, -4),
+                            (12, 68, -4), (18, 128, -4), (8, 256, -4)):
+        bad = list(ok)
+        bad[at] = value
+        assert L.h3_gemm_adapters(*bad) == code, (at, value)
+    assert L.h3_gemm_adapters(*ok) == -12  # no workspace bytes
+    need = L.h3_gemm_adapters_workspace(300, 1, 512, 256, 0, 16, 4)
+    assert need >= 300 * 16 * 2
+    assert L.h3_gemm_adapters_workspace(0, 1, 512, 256, 0, 16, 4) == -3
+    assert L.h3_gemm_adapters_workspace(300, 1, 512, 256, 0, 24, 4) == -3
+    assert L.h3_gemm_adapters_workspace(300, 1, 1 << 24, 1 << 30, 1, 16, 4) == -3
+
+
+def test_stack_adapters():
+    import h3attn as O
+    A = [torch.randn(r, 40) for r in (3, 20)]
+    B = [torch.randn(16, r) for r in (3, 20)]
+    a, b, s = O.stack_adapters(zip(A, B), [1, 0.5])
+    assert a.shape == (64, 40) and b.shape == (16, 64) and s.tolist() == [1.0, 0.5]
+    assert torch.equal(a[:3], A[0].bfloat16()) and not a[3:32].any() and torch.equal(a[32:52], A[1].bfloat16())
+    assert torch.equal(b[:, 32:52], B[1].bfloat16()) and not b[:, 52:].any()
+    for bad in (([], []), ([(A[0], B[0])], [1, 2]), ([(A[0], B[1])], [1]), ([(torch.zeros(300, 8), torch.zeros(8, 300))], [1])):
+        with pytest.raises(O.H3Error):
+            O.stack_adapters(*bad)
+
+
+@pytest.mark.parametrize("tiles,n_kb,ctas", [(1, 1, 296), (171, 84, 296), (43, 112, 296), (253, 4, 296), (9, 3, 8),
+                                             (2, 1000, 7)])
+def test_streamed_blocks_are_dealt_once(tiles, n_kb, ctas):
+    """The row path's split of (tile, k-block) over CTAs, restated: every block in one CTA, a tile's pieces numbered
+    from 0 without gaps, and never more of them than the workspace holds."""
+    total = tiles * n_kb
+    per = -(-total // ctas)
+    most = (n_kb + per - 2) // per + 1
+    seen = set()
+    for cta in range(-(-total // per)):
+        g = cta * per
+        while g < min(total, (cta + 1) * per):
+            tile, kb0 = divmod(g, n_kb)
+            kb1 = min(n_kb, kb0 + min(total, (cta + 1) * per) - g)
+            piece = cta - tile * n_kb // per
+            count = ((tile + 1) * n_kb - 1) // per - tile * n_kb // per + 1
+            assert 0 <= piece < count <= most
+            for kb in range(kb0, kb1):
+                assert (tile, kb) not in seen
+                seen.add((tile, kb))
+            g += kb1 - kb0
+    assert len(seen) == total
