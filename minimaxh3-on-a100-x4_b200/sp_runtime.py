@@ -13,6 +13,13 @@ Same module API and behaviour, B200 data path underneath:
   env SP_OVERLAP=heads         head-by-head all-to-all / attention pipelining (this build)
   env SP_OVERLAP=peer          all-to-alls fused into pack / attention over peer memory (this build)
   env SP_OVERLAP=ce            all-to-alls as copy-engine copies into peers' final buffers (this build)
+  rope_freqs                   may be an h3attn.RopePositions: rotary angles from (time, height, width) positions,
+                               computed inside the pack kernel (this build)
+  transformer_options["h3_window"] = {"left": n, "right": n, "sinks": n}
+                               attention over a sliding window, the first `sinks` tokens (the prompt) visible to all;
+                               a missing or None side has no bound (this build; not with SP_OVERLAP=peer)
+  set_adapters(linear, stacked), transformer_options["h3_adapter_segments"] = [(a, b, adapter), ...]
+                               low-rank adapters of token segments on the block's projections (this build)
 
 What differs, by design:
   * The attention layer runs on libh3attn.so (sm_100a): one fused kernel does the q/k
@@ -65,6 +72,9 @@ _orig_attn_forward = None
 _orig_run_blocks = None
 _orig_mlp_forward = None
 _MODULE = None
+
+# int32 adapter of each local token while run_blocks runs with "h3_adapter_segments", else None
+_ADAPTER_ROWS = None
 
 _ops = None  # the kernel library binding (h3attn); resolved on first use
 
@@ -172,9 +182,57 @@ def _h3sla_schedule(transformer_options):
     return None
 
 
+def _is_positions(rope_freqs) -> bool:
+    """rope_freqs is an h3attn.RopePositions, not a table of rotation matrices."""
+    return hasattr(rope_freqs, "inv_freq")
+
+
+def _window(transformer_options):
+    """(left, right, sinks) of transformer_options["h3_window"], or None for dense attention."""
+    w = (transformer_options or {}).get("h3_window")
+    if w is None:
+        return None
+    unknown = set(w) - {"left", "right", "sinks"}
+    if unknown:
+        raise ValueError(f"h3_window: unknown keys {sorted(unknown)}")
+    return w.get("left"), w.get("right"), int(w.get("sinks") or 0)
+
+
+def _attend(O, window, q, k, v, s_kv, layout, world=1):
+    """The layer's attention over whole sequences of queries: dense, or over a window (in one split of the keys, so
+    that a row's bits do not depend on how many heads this rank has)."""
+    if window is None:
+        return O.attention(q, k, v, s_kv=s_kv, layout=layout, world=world)
+    left, right, sinks = window
+    return O.window_attention(q, k, v, left, right, sinks=sinks, q_start=0, s_kv=s_kv, layout=layout, world=world,
+                              splits=1)
+
+
+def set_adapters(linear, stacked) -> None:
+    """Attach low-rank adapters to a projection of the host model (qkv_proj, out_proj, fc1 or fc2): stacked =
+    (lora_a, lora_b, scale) of h3attn.stack_adapters, or None to take them off. They act in run_blocks calls that
+    name token segments in transformer_options["h3_adapter_segments"]."""
+    if stacked is None:
+        if hasattr(linear, "h3_adapters"):
+            del linear.h3_adapters
+    else:
+        lora_a, lora_b, scale = stacked
+        linear.h3_adapters = (lora_a, lora_b, scale)
+
+
+def _project(O, lin, a, w, epilogue="none"):
+    """a @ w.T on the library's GEMM, with the projection's adapters where this call has adapter rows."""
+    ad = getattr(lin, "h3_adapters", None)
+    if ad is None or _ADAPTER_ROWS is None:
+        return O.linear(a, w) if epilogue == "none" else O.linear(a, w, epilogue=epilogue)
+    return O.linear_lora(a, w, *ad, _ADAPTER_ROWS, epilogue=epilogue)
+
+
 def _norm_inputs(self, x, rope_freqs):
     rope = None
-    if rope_freqs is not None:
+    if _is_positions(rope_freqs):
+        rope = rope_freqs
+    elif rope_freqs is not None:
         rot = rope_freqs.shape[-3] * 2
         if rot != self.head_dim:
             raise NotImplementedError(f"rotary dim {rot} != head_dim {self.head_dim} is not supported")
@@ -220,6 +278,8 @@ def _gemm_weight(lin, x):
     elif w.dim() != 2 or w.device != x.device:
         why = "weight shape or device"
     if why is not None:
+        if _ADAPTER_ROWS is not None and getattr(lin, "h3_adapters", None) is not None:
+            raise RuntimeError(f"sp_runtime: a projection with adapters cannot run on the library's GEMM ({why})")
         if x.is_cuda:
             _host_fallback("a projection", why)
         return None
@@ -233,7 +293,7 @@ def _sp_mlp_forward(self, x):
     if not _SP_ACTIVE or w1 is None or w2 is None or x.dim() != 2:
         return _orig_mlp_forward(self, x)
     O = ops()
-    return O.linear(O.linear(x, w1, epilogue="swiglu"), w2)
+    return _project(O, self.fc2, _project(O, self.fc1, x, w1, "swiglu"), w2)
 
 
 def _sp_attn_forward(self, x, rope_freqs=None, transformer_options={}):
@@ -244,7 +304,7 @@ def _sp_attn_forward(self, x, rope_freqs=None, transformer_options={}):
     H, D, W = self.heads, self.head_dim, WORLD
     with _span("qkv"):
         w_qkv = _gemm_weight(self.qkv_proj, x)
-        qkv = O.linear(x, w_qkv) if w_qkv is not None else self.qkv_proj(x)
+        qkv = _project(O, self.qkv_proj, x, w_qkv) if w_qkv is not None else self.qkv_proj(x)
         q, k, v = qkv.split(H * D, dim=-1)
         rope, qw, kw = _norm_inputs(self, x, rope_freqs)
         send = O.qknorm_rope_pack(q, k, v, rope, qw, kw, self.q_norm.eps, W)  # [W, 3, H/W, s, D]
@@ -253,10 +313,11 @@ def _sp_attn_forward(self, x, rope_freqs=None, transformer_options={}):
     with _span("fa2_local"):
         S_pad = W * s
         s_kv = _SP_REAL_S if (_SP_REAL_S is not None and _SP_REAL_S < S_pad) else S_pad
+        window = _window(transformer_options)
         if W > 1:
-            o_send = O.attention(qkvh[0], qkvh[1], qkvh[2], s_kv=s_kv, layout="send", world=W)
+            o_send = _attend(O, window, qkvh[0], qkvh[1], qkvh[2], s_kv, "send", W)
         else:
-            o = O.attention(qkvh[0], qkvh[1], qkvh[2], s_kv=s_kv, layout="token")
+            o = _attend(O, window, qkvh[0], qkvh[1], qkvh[2], s_kv, "token")
     with _span("a2a_inv"):
         if W > 1:
             o_recv = _exchange(o_send)  # [W, H/W, s, D] == [H, s, D]
@@ -265,9 +326,9 @@ def _sp_attn_forward(self, x, rope_freqs=None, transformer_options={}):
         if W > 1:
             o_heads = o_recv.view(H, s, D)
             if w_out is not None:
-                return O.linear(o_heads, w_out)  # reads [H, s, D] as [s, H*D] in place
+                return _project(O, self.out_proj, o_heads, w_out)  # reads [H, s, D] as [s, H*D] in place
             o = O.head_to_seq_unpack(o_heads)
-        return O.linear(o, w_out) if w_out is not None else self.out_proj(o)
+        return _project(O, self.out_proj, o, w_out) if w_out is not None else self.out_proj(o)
 
 
 # ---- comm/compute overlap (exact): Q and O exchanged in token pieces on a side stream ----
@@ -300,7 +361,7 @@ def _sp_attn_forward_overlap(self, x, rope_freqs=None, transformer_options={}):
     s = x.shape[0]
     H, D, W = self.heads, self.head_dim, WORLD
     w_qkv = _gemm_weight(self.qkv_proj, x)
-    qkv = O.linear(x, w_qkv) if w_qkv is not None else self.qkv_proj(x)
+    qkv = _project(O, self.qkv_proj, x, w_qkv) if w_qkv is not None else self.qkv_proj(x)
     q, k, v = qkv.split(H * D, dim=-1)
     rope, qw, kw = _norm_inputs(self, x, rope_freqs)
     send = O.qknorm_rope_pack(q, k, v, rope, qw, kw, self.q_norm.eps, W)  # [W, 3, H/W, s, D]
@@ -308,6 +369,7 @@ def _sp_attn_forward_overlap(self, x, rope_freqs=None, transformer_options={}):
     S_pad = W * s
     s_kv = _SP_REAL_S if (_SP_REAL_S is not None and _SP_REAL_S < S_pad) else S_pad
     pieces = _piece_bounds(s, _PIECES)
+    window = _window(transformer_options)
     default = torch.cuda.current_stream()
     _comm_stream.wait_stream(default)
     o = torch.empty((s, H * D), dtype=x.dtype, device=x.device)
@@ -325,14 +387,21 @@ def _sp_attn_forward_overlap(self, x, rope_freqs=None, transformer_options={}):
         if i + 1 < len(pieces):
             with torch.cuda.stream(_comm_stream):
                 qh_next = q_piece(*pieces[i + 1])
-        o_send = O.attention(qh_p, kvh[0], kvh[1], s_kv=s_kv, layout="send", world=W)
+        if window is None:
+            o_send = O.attention(qh_p, kvh[0], kvh[1], s_kv=s_kv, layout="send", world=W)
+        else:  # the piece holds rows [lo, hi) of every rank's shard: one run of positions per rank
+            n = hi - lo
+            o_send = torch.empty((W, H // W, n, D), dtype=x.dtype, device=x.device)
+            for r in range(W):
+                O.window_attention(qh_p[:, r * n:(r + 1) * n], kvh[0], kvh[1], window[0], window[1], sinks=window[2],
+                                   q_start=r * s + lo, s_kv=s_kv, splits=1, out=o_send[r])
         with torch.cuda.stream(_comm_stream):
             _comm_stream.wait_stream(default)
             o_send.record_stream(_comm_stream)
             O.head_to_seq_unpack(_exchange(o_send).view(H, hi - lo, D), out=o[lo:hi])
     default.wait_stream(_comm_stream)
     w_out = _gemm_weight(self.out_proj, x)
-    return O.linear(o, w_out) if w_out is not None else self.out_proj(o)
+    return _project(O, self.out_proj, o, w_out) if w_out is not None else self.out_proj(o)
 
 
 def _sp_attn_forward_heads(self, x, rope_freqs=None, transformer_options={}):
@@ -357,13 +426,14 @@ def _sp_attn_forward_heads(self, x, rope_freqs=None, transformer_options={}):
     hl = H // W
     with _span("qkv"):
         w_qkv = _gemm_weight(self.qkv_proj, x)
-        qkv = O.linear(x, w_qkv) if w_qkv is not None else self.qkv_proj(x)
+        qkv = _project(O, self.qkv_proj, x, w_qkv) if w_qkv is not None else self.qkv_proj(x)
         q, k, v = qkv.split(H * D, dim=-1)
         rope, qw, kw = _norm_inputs(self, x, rope_freqs)
         send = O.qknorm_rope_pack(q, k, v, rope, qw, kw, self.q_norm.eps, W, head_major=True)  # [hl, W, 3, s, D]
     S_pad = W * s
     s_kv = _SP_REAL_S if (_SP_REAL_S is not None and _SP_REAL_S < S_pad) else S_pad
     default = torch.cuda.current_stream()
+    window = _window(transformer_options)
     o_heads = torch.empty((W, hl, s, D), dtype=x.dtype, device=x.device)  # == [H, s, D], head g = src*hl + h
     with _span("fa2_local"):
         _comm_stream.wait_stream(default)
@@ -382,7 +452,7 @@ def _sp_attn_forward_heads(self, x, rope_freqs=None, transformer_options={}):
             recvs[h].record_stream(cs)
             with torch.cuda.stream(cs):
                 qkvh = O.seq_to_head_unpack(recvs[h].view(W, 3, 1, s, D))  # [3, 1, W*s, D]
-                o_send = O.attention(qkvh[0], qkvh[1], qkvh[2], s_kv=s_kv, layout="send", world=W)  # [W, 1, s, D]
+                o_send = _attend(O, window, qkvh[0], qkvh[1], qkvh[2], s_kv, "send", W)  # [W, 1, s, D]
                 done = torch.cuda.Event()
                 done.record(cs)
             o_send.record_stream(_comm_stream)
@@ -394,7 +464,7 @@ def _sp_attn_forward_heads(self, x, rope_freqs=None, transformer_options={}):
     with _span("out_proj"):
         w_out = _gemm_weight(self.out_proj, x)
         o_hsd = o_heads.view(H, s, D)
-        return O.linear(o_hsd, w_out) if w_out is not None else self.out_proj(O.head_to_seq_unpack(o_hsd))
+        return _project(O, self.out_proj, o_hsd, w_out) if w_out is not None else self.out_proj(O.head_to_seq_unpack(o_hsd))
 
 
 _peer_cache = {}
@@ -453,6 +523,8 @@ def _sp_attn_forward_peer(self, x, rope_freqs=None, transformer_options={}):
         return _orig_attn_forward(self, x, rope_freqs=rope_freqs, transformer_options=transformer_options)
     if WORLD == 1:
         return _sp_attn_forward(self, x, rope_freqs=rope_freqs, transformer_options=transformer_options)
+    if _window(transformer_options) is not None:
+        raise NotImplementedError("SP_OVERLAP=peer runs dense attention: use another mode with h3_window")
     O = ops()
     s = x.shape[0]
     H, D, W = self.heads, self.head_dim, WORLD
@@ -462,7 +534,7 @@ def _sp_attn_forward_peer(self, x, rope_freqs=None, transformer_options={}):
     s_kv = _SP_REAL_S if (_SP_REAL_S is not None and _SP_REAL_S < S_pad) else S_pad
     with _span("qkv"):
         w_qkv = _gemm_weight(self.qkv_proj, x)
-        qkv = O.linear(x, w_qkv) if w_qkv is not None else self.qkv_proj(x)
+        qkv = _project(O, self.qkv_proj, x, w_qkv) if w_qkv is not None else self.qkv_proj(x)
         q, k, v = qkv.split(H * D, dim=-1)
         rope, qw, kw = _norm_inputs(self, x, rope_freqs)
         O.qknorm_rope_pack_peer(q, k, v, rope, qw, kw, self.q_norm.eps, W, buf["qkv_ptrs"], hl * S_pad * D,
@@ -476,7 +548,7 @@ def _sp_attn_forward_peer(self, x, rope_freqs=None, transformer_options={}):
         _peer_barrier(buf["flag"])  # every rank's output rows for this rank have landed
     with _span("out_proj"):
         w_out = _gemm_weight(self.out_proj, x)
-        return O.linear(buf["o"], w_out) if w_out is not None else self.out_proj(buf["o"].clone())
+        return _project(O, self.out_proj, buf["o"], w_out) if w_out is not None else self.out_proj(buf["o"].clone())
 
 
 _ce_streams = {}
@@ -534,7 +606,7 @@ def _sp_attn_forward_ce(self, x, rope_freqs=None, transformer_options={}):
     s_kv = _SP_REAL_S if (_SP_REAL_S is not None and _SP_REAL_S < S_pad) else S_pad
     with _span("qkv"):
         w_qkv = _gemm_weight(self.qkv_proj, x)
-        qkv = O.linear(x, w_qkv) if w_qkv is not None else self.qkv_proj(x)
+        qkv = _project(O, self.qkv_proj, x, w_qkv) if w_qkv is not None else self.qkv_proj(x)
         q, k, v = qkv.split(H * D, dim=-1)
         rope, qw, kw = _norm_inputs(self, x, rope_freqs)
         send = O.qknorm_rope_pack(q, k, v, rope, qw, kw, self.q_norm.eps, W)  # [W, 3, H/W, s, D]
@@ -545,7 +617,7 @@ def _sp_attn_forward_ce(self, x, rope_freqs=None, transformer_options={}):
         _peer_barrier(buf["flag"])  # every rank's q/k/v rows have landed
     with _span("fa2_local"):
         qkvh = buf["qkv"]
-        o_send = O.attention(qkvh[0], qkvh[1], qkvh[2], s_kv=s_kv, layout="send", world=W)  # [W, H/W, s, D]
+        o_send = _attend(O, _window(transformer_options), qkvh[0], qkvh[1], qkvh[2], s_kv, "send", W)  # [W, H/W, s, D]
     with _span("a2a_inv"):
         off, blk = geo["o"]
         _ce_copies(buf["o_base"], off, blk, o_send, blk, 1, x.device)
@@ -554,7 +626,7 @@ def _sp_attn_forward_ce(self, x, rope_freqs=None, transformer_options={}):
         o_heads = buf["o"].view(H, s, D)
         w_out = _gemm_weight(self.out_proj, x)
         if w_out is not None:
-            return O.linear(o_heads, w_out)  # reads [H, s, D] as [s, H*D] in place
+            return _project(O, self.out_proj, o_heads, w_out)  # reads [H, s, D] as [s, H*D] in place
         return self.out_proj(O.head_to_seq_unpack(o_heads))
 
 
@@ -645,27 +717,33 @@ def _shard_bounds(S: int, world: int, rank: int) -> tuple[int, int, int]:
 
 
 def _sp_run_blocks(self, h, t_emb, mod_segments, rope_freqs, transformer_options={}):
-    global _SP_ACTIVE, _SP_REAL_S, _timeline
+    global _SP_ACTIVE, _SP_REAL_S, _ADAPTER_ROWS, _timeline
     S = h.shape[0]
     S_pad, lo, hi = _shard_bounds(S, WORLD, RANK)
     # Pad rows sit after the last token: they belong to no modulation segment (scale, shift and
     # gate leave them alone), their keys are cut off inside attention (_SP_REAL_S), and the
     # all-gather's tail drops them again.
     h_loc = h[lo:min(hi, S)]
-    rope_loc = rope_freqs[:, lo:min(hi, S)] if rope_freqs is not None else None
+    table = rope_freqs is not None and not _is_positions(rope_freqs)
+    rope_loc = rope_freqs[:, lo:min(hi, S)] if table else None
     if hi > S:
         h_loc = torch.cat([h_loc, h.new_zeros(hi - max(lo, S), h.shape[1])], dim=0)
-        if rope_freqs is not None:
+        if table:
             tail = rope_freqs.new_zeros((rope_freqs.shape[0], hi - max(lo, S)) + tuple(rope_freqs.shape[2:]))
             rope_loc = torch.cat([rope_loc, tail], dim=1)
     h_loc = h_loc.contiguous()
     rope_loc = rope_loc.contiguous() if rope_loc is not None else None
+    if _is_positions(rope_freqs):
+        rope_loc = rope_freqs.rows(lo, hi)
     segs_loc = _shard_segments(mod_segments, lo, hi)
     host_block = _host_block_timed if _TIMING else None
     _timeline = _Timeline(h_loc.is_cuda) if _TIMING else None
     _SP_ACTIVE, _SP_REAL_S = True, S
     seg_row = None
     try:
+        adapter_segs = (transformer_options or {}).get("h3_adapter_segments")
+        if adapter_segs:
+            _ADAPTER_ROWS = ops().segment_rows(_shard_segments(adapter_segs, lo, hi), h_loc.shape[0], h_loc.device)
         for blk in self.blocks:
             if _fusable(blk, h_loc):
                 if seg_row is None:
@@ -678,7 +756,7 @@ def _sp_run_blocks(self, h, t_emb, mod_segments, rope_freqs, transformer_options
         with _span("gather"):
             out = _gather_rows(h_loc) if WORLD > 1 else h_loc
     finally:
-        _SP_ACTIVE, _SP_REAL_S = False, None
+        _SP_ACTIVE, _SP_REAL_S, _ADAPTER_ROWS = False, None, None
         timeline, _timeline = _timeline, None
     if timeline is not None:
         _last_totals.clear()
