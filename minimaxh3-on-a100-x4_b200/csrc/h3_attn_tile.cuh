@@ -92,19 +92,6 @@ __device__ __forceinline__ void issue_pv_steps(uint32_t d_tmem, uint32_t p_tmem,
   }
 }
 
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-inline EncodeTiledFn get_encode_fn() {
-  void* fn = nullptr;
-  cudaDriverEntryPointQueryResult qres;
-  if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qres) != cudaSuccess ||
-      qres != cudaDriverEntryPointSuccess)
-    return nullptr;
-  return reinterpret_cast<EncodeTiledFn>(fn);
-}
-
 // [n_heads][rows][128] bf16 with element strides (row_stride, head_stride); box 64 x box_rows x 1, SW128.
 inline int make_head_map(CUtensorMap* map, const void* base, long long rows, long long n_heads,
                          long long row_stride, long long head_stride, unsigned box_rows = 128) {

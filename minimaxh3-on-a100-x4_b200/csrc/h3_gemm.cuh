@@ -391,23 +391,16 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmap_a, const CUten
 }
 
 // ---------------------------------------------------------------- host
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
 // [outer][rows][inner] bf16 with element strides; box 64 x box_rows x 1, SW128, zero fill out of range.
 inline int make_map(CUtensorMap* map, const void* base, long long inner, long long rows, long long outer,
                     long long row_stride, long long outer_stride, unsigned box_rows = 128) {
-  void* fn = nullptr;
-  cudaDriverEntryPointQueryResult qres;
-  if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qres) != cudaSuccess ||
-      qres != cudaDriverEntryPointSuccess)
-    return H3_ERR_DRIVER;
+  const EncodeTiledFn enc = get_encode_fn();
+  if (!enc) return H3_ERR_DRIVER;
   cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)outer};
   cuuint64_t strides[2] = {(cuuint64_t)row_stride * 2, (cuuint64_t)outer_stride * 2};
   cuuint32_t box[3] = {64, box_rows, 1};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = reinterpret_cast<EncodeTiledFn>(fn)(
+  CUresult r = enc(
       map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

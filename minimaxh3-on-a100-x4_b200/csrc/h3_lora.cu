@@ -572,23 +572,6 @@ static int make_layout(int64_t m, int64_t n_kb, int64_t kc_blocks, int64_t w_row
   return H3_OK;
 }
 
-// Launch as a programmatic dependent of the kernel before it on the stream.
-template <typename... P, typename... A>
-static int launch_dependent(void (*kern)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) return H3_ERR_LAUNCH;
-  return cudaGetLastError() == cudaSuccess ? H3_OK : H3_ERR_LAUNCH;
-}
-
 template <typename K>
 static int allow_smem(K* kern, uint32_t bytes) {
   return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess

@@ -1,7 +1,8 @@
 // Helpers of the kernels that walk 128-element bf16 head rows (pack, rotary): 16-byte vectors of eight
-// bf16 to fp32 and back, launch sizing and the pointer check.
+// bf16 to fp32 and back, launch sizing, the pointer check and the tensor-map encoder.
 #pragma once
 #include "h3_ptx.cuh"
+#include "h3attn.h"
 
 namespace h3 {
 
@@ -24,11 +25,45 @@ __device__ __forceinline__ uint4 f32_to_bf16x8(const float* f) {
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The driver's cuTensorMapEncodeTiled, looked up once per process (the lookup costs more than a call).
+inline EncodeTiledFn get_encode_fn() {
+  static const EncodeTiledFn found = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult qres;
+    return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qres) == cudaSuccess &&
+                   qres == cudaDriverEntryPointSuccess
+               ? reinterpret_cast<EncodeTiledFn>(fn)
+               : nullptr;
+  }();
+  return found;
+}
+
 inline int grid_for(long long work_items, int per_block, int max_blocks) {
   long long b = (work_items + per_block - 1) / per_block;
   if (b < 1) b = 1;
   if (b > max_blocks) b = max_blocks;
   return (int)b;
+}
+
+// Launch as a programmatic dependent of the kernel before it on the stream.
+template <typename... P, typename... A>
+int launch_dependent(void (*kern)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) return H3_ERR_LAUNCH;
+  return cudaGetLastError() == cudaSuccess ? H3_OK : H3_ERR_LAUNCH;
 }
 
 }  // namespace h3

@@ -130,7 +130,9 @@ def _check(rc: int, what: str) -> None:
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    """The raw handle of the current stream (torch.cuda.current_stream() builds a Stream object around it, which
+    costs 3 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _cuda(t: torch.Tensor, name: str, dtype=torch.bfloat16) -> None:
@@ -140,17 +142,25 @@ def _cuda(t: torch.Tensor, name: str, dtype=torch.bfloat16) -> None:
         raise H3Error(f"{name} must be {dtype}, got {t.dtype}")
 
 
-def _together(dev, **tensors) -> None:
-    """Every given tensor lives on `dev`."""
+def _together(index: int, **tensors) -> None:
+    """Every given tensor lives on GPU `index`."""
     for n, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise H3Error(f"{n} is on {t.device}, the call runs on {dev}")
+        if t is not None and t.get_device() != index:
+            raise H3Error(f"{n} is on {t.device}, the call runs on cuda:{index}")
 
 
-def _on(dev):
-    """Context in which `dev` is the current device: a launch goes to its tensors' device, on the
+_HERE = contextlib.nullcontext()
+
+
+def _on(index: int):
+    """Context in which GPU `index` is the current device: a launch goes to its tensors' device, on the
     stream that is current there."""
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    return _HERE if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def _status_ptr(index: int) -> int:
+    st = _status.get(index)
+    return (st if st is not None else status_word(torch.device("cuda", index))).data_ptr()
 
 
 def status_word(device=None) -> torch.Tensor:
@@ -243,6 +253,12 @@ def _window_plan(dev_index: int, *shape) -> tuple:
     return rc, n.value
 
 
+def _head_strides(t: torch.Tensor, heads: int, rows: int) -> tuple:
+    """(head, row) strides of [heads, rows, 128]; an axis of one element has whatever stride, 128 stands for it."""
+    st = t.stride()
+    return st[0] if heads > 1 else D, st[1] if rows > 1 else D
+
+
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: int | None, right: int | None,
                      sinks: int = 0, causal: bool = False, q_start: int | None = None, s_kv: int | None = None,
                      scale: float | None = None, out: torch.Tensor | None = None, layout: str = "head",
@@ -259,14 +275,14 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: in
         _cuda(t, n)
         if t.dim() != 3 or t.shape[-1] != D or t.stride(-1) != 1:
             raise H3Error(f"{n} must be [heads, rows, 128] with a contiguous last dim, got {tuple(t.shape)}")
-    dev = q.device
+    dev = q.get_device()
     _together(dev, k=k, v=v, out=out)
     H, sq, _ = q.shape
     hk, skv_alloc, _ = k.shape
     if v.shape != k.shape or hk < 1 or H % hk:
         raise H3Error("k and v must share a shape, and the query heads be a multiple of the key heads")
-    q_st, k_st, v_st = (tuple(t.stride(i) if t.shape[i] > 1 else D for i in (0, 1)) for t in (q, k, v))
-    if k_st != v_st:
+    q_st, k_st = _head_strides(q, H, sq), _head_strides(k, hk, skv_alloc)
+    if _head_strides(v, hk, skv_alloc) != k_st:
         raise H3Error("k and v must share strides")
     s_kv = skv_alloc if s_kv is None else int(s_kv)
     if not 1 <= s_kv <= skv_alloc:
@@ -280,7 +296,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: in
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     shape, rank_rows, rank_stride, head_stride, row_stride = _out_layout(layout, H, sq, world)
     if out is None:
-        out = torch.empty(shape, dtype=torch.bfloat16, device=dev)
+        out = q.new_empty(shape)
     else:
         _cuda(out, "out")
         if tuple(out.shape) != tuple(shape) or not out.is_contiguous():
@@ -290,12 +306,12 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: in
     lo, hi = (-1 if side is None or side > big else int(side) for side in (left, right))
     sinks = min(int(sinks), s_kv)
     with _on(dev):
-        n_splits, ws_bytes = _window_plan(dev.index, H, hk, sq, s_kv, lo, hi, sinks, int(causal), q_start, splits or 0)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+        n_splits, ws_bytes = _window_plan(dev, H, hk, sq, s_kv, lo, hi, sinks, int(causal), q_start, splits or 0)
+        ws = q.new_empty((ws_bytes // 2,)) if ws_bytes else None
         rc = lib().h3_window_attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), H, hk, sq, s_kv,
                                   *q_st, *k_st, rank_rows, rank_stride,
                                   head_stride, row_stride, scale, lo, hi, sinks, int(causal), q_start, n_splits,
-                                  ws.data_ptr() if ws_bytes else None, ws_bytes, status_word(dev).data_ptr(), _stream())
+                                  ws.data_ptr() if ws_bytes else None, ws_bytes, _status_ptr(dev), _stream())
     _check(rc, "h3_window_attn")
     return out
 
@@ -318,6 +334,9 @@ def rope_axes_freqs(sections, theta: float = 10000.0, interleaved: bool = False,
             torch.tensor([a for _, a in pairs] + [-1] * rest, dtype=torch.int32, device=device))
 
 
+_PAIRS = torch.Size([D // 2])
+
+
 class RopePositions:
     """Positions of tokens on several axes and the frequencies that turn them:
       pos: [tokens, axes] int32 or fp32; inv_freq: fp64 [64] radians per unit position of pair (i, i + 64);
@@ -338,20 +357,20 @@ class RopePositions:
             pos = torch.cat([pos, pos.new_zeros((hi - lo - pos.shape[0],) + tuple(pos.shape[1:]))])
         return RopePositions(pos.contiguous(), self.inv_freq, self.axis)
 
-    def _args(self, tokens: int, dev) -> tuple:
+    def _args(self, tokens: int, index: int) -> tuple:
         """(pos, type, axes, inv_freq, axis) for the C calls, checked."""
         pos, f, a = self.pos, self.inv_freq, self.axis
-        for n, t, dt in (("inv_freq", f, torch.float64), ("axis", a, torch.int32)):
-            _cuda(t, n, dt)
-            if tuple(t.shape) != (D // 2,) or not t.is_contiguous():
-                raise H3Error(f"{n} must be contiguous [{D // 2}]")
-        if not isinstance(pos, torch.Tensor) or pos.dtype not in (torch.int32, torch.float32):
-            raise H3Error("pos must be an int32 or fp32 tensor")
-        _cuda(pos, "pos", pos.dtype)
-        if pos.dim() != 2 or pos.shape[0] != tokens or not 1 <= pos.shape[1] <= 64 or not pos.is_contiguous():
-            raise H3Error(f"pos must be contiguous [{tokens}, axes] with 1 to 64 axes, got {tuple(pos.shape)}")
-        _together(dev, pos=pos, inv_freq=f, axis=a)
-        return pos.data_ptr(), int(pos.dtype == torch.float32), pos.shape[1], f.data_ptr(), a.data_ptr()
+        _cuda(f, "inv_freq", torch.float64)
+        _cuda(a, "axis", torch.int32)
+        if f.shape != _PAIRS or a.shape != _PAIRS or not (f.is_contiguous() and a.is_contiguous()):
+            raise H3Error(f"inv_freq and axis must be contiguous [{D // 2}]")
+        real = isinstance(pos, torch.Tensor) and pos.dtype == torch.float32
+        _cuda(pos, "pos", torch.float32 if real else torch.int32)
+        shape = pos.shape
+        if len(shape) != 2 or shape[0] != tokens or not 1 <= shape[1] <= 64 or not pos.is_contiguous():
+            raise H3Error(f"pos must be contiguous [{tokens}, axes] with 1 to 64 axes, got {tuple(shape)}")
+        _together(index, pos=pos, inv_freq=f, axis=a)
+        return pos.data_ptr(), int(real), shape[1], f.data_ptr(), a.data_ptr()
 
 
 def rope_axes(x: torch.Tensor, positions: RopePositions, inverse: bool = False,
@@ -363,16 +382,18 @@ def rope_axes(x: torch.Tensor, positions: RopePositions, inverse: bool = False,
     if x.dim() != 3 or x.shape[-1] != D or x.stride(-1) != 1:
         raise H3Error(f"x must be [tokens, heads, 128] with a contiguous last dim, got {tuple(x.shape)}")
     if out is None:
-        out = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
+        out = x.new_empty(x.shape)
     else:
         _cuda(out, "out")
         if out.shape != x.shape or out.stride(-1) != 1:
             raise H3Error(f"out must be {tuple(x.shape)} with a contiguous last dim")
-        _together(x.device, out=out)
-    args = positions._args(x.shape[0], x.device)
-    with _on(x.device):
-        rc = lib().h3_rope_axes(x.data_ptr(), x.stride(0), x.stride(1), *args, int(inverse), out.data_ptr(),
-                                out.stride(0), out.stride(1), x.shape[0], x.shape[1], _stream())
+    tokens, heads, _ = x.shape
+    dev, x_st, o_st = x.get_device(), x.stride(), out.stride()
+    _together(dev, out=out)
+    args = positions._args(tokens, dev)
+    with _on(dev):
+        rc = lib().h3_rope_axes(x.data_ptr(), x_st[0], x_st[1], *args, int(inverse), out.data_ptr(), o_st[0], o_st[1],
+                                tokens, heads, _stream())
     _check(rc, "h3_rope_axes")
     return out
 
@@ -392,10 +413,11 @@ def qknorm_rope_pack_peer(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rop
     if tuple(rank_base.shape) != (world,) or not rank_base.is_contiguous():
         raise H3Error("rank_base must be a contiguous int64 [world] device tensor")
     if axes is not None:
-        _together(q.device, k=k, v=v, q_weight=q_weight, k_weight=k_weight, rank_base=rank_base)
-        with _on(q.device):
+        dev = q.get_device()
+        _together(dev, k=k, v=v, q_weight=q_weight, k_weight=k_weight, rank_base=rank_base)
+        with _on(dev):
             rc = lib().h3_qknorm_rope_pack_axes_peer(
-                q2.data_ptr(), k2.data_ptr(), v2.data_ptr(), q2.stride(0), *axes._args(sl, q.device), wptr[0], wptr[1],
+                q2.data_ptr(), k2.data_ptr(), v2.data_ptr(), q2.stride(0), *axes._args(sl, dev), wptr[0], wptr[1],
                 float(eps), rank_base.data_ptr(), world, tensor_stride, head_stride, row_offset, sl, H, H // world,
                 _stream())
         _check(rc, "h3_qknorm_rope_pack_axes_peer")
@@ -493,10 +515,11 @@ def qknorm_rope_pack(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, rope: to
     base = out.data_ptr()
     if axes is not None:
         _cuda(out, "out")
-        _together(q.device, k=k, v=v, q_weight=q_weight, k_weight=k_weight, out=out)
-        with _on(q.device):
+        dev = q.get_device()
+        _together(dev, k=k, v=v, q_weight=q_weight, k_weight=k_weight, out=out)
+        with _on(dev):
             rc = lib().h3_qknorm_rope_pack_axes(
-                q2.data_ptr(), k2.data_ptr(), v2.data_ptr(), q2.stride(0), *axes._args(sl, q.device), wptr[0], wptr[1],
+                q2.data_ptr(), k2.data_ptr(), v2.data_ptr(), q2.stride(0), *axes._args(sl, dev), wptr[0], wptr[1],
                 float(eps), base, base + 2 * tstride, base + 4 * tstride, sl, H, hl, rank_stride, head_stride,
                 _stream())
         _check(rc, "h3_qknorm_rope_pack_axes")
@@ -579,7 +602,7 @@ def _linear_args(a, weight, out, epilogue):
     if ep == 1 and weight.shape[0] % 2:
         raise H3Error("swiglu weight needs an even row count")
     if out is None:
-        out = torch.empty((m, n), dtype=torch.bfloat16, device=a.device)
+        out = a.new_empty((m, n))
     else:
         _cuda(out, "out")
         if tuple(out.shape) != (m, n) or out.stride(-1) != 1:
@@ -654,26 +677,26 @@ def linear_lora(a: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
     _cuda(lora_b, "lora_b")
     _cuda(scale, "scale", torch.float32)
     _cuda(rows, "rows", torch.int32)
-    dev = a.device
+    dev = a.get_device()
     _together(dev, weight=weight, lora_a=lora_a, lora_b=lora_b, scale=scale, rows=rows, out=out)
     if scale.dim() != 1 or scale.shape[0] < 1 or not scale.is_contiguous():
         raise H3Error("scale must be a contiguous fp32 [adapters]")
     n_adapters = scale.shape[0]
     if lora_a.dim() != 2 or lora_a.shape[1] != weight.shape[1] or lora_a.shape[0] % n_adapters or lora_a.stride(1) != 1:
         raise H3Error(f"lora_a must be [{n_adapters} * rank, {weight.shape[1]}] with a contiguous last dim")
-    if tuple(lora_b.shape) != (weight.shape[0], lora_a.shape[0]) or lora_b.stride(1) != 1:
+    if lora_b.shape != (weight.shape[0], lora_a.shape[0]) or lora_b.stride(1) != 1:
         raise H3Error(f"lora_b must be [{weight.shape[0]}, {lora_a.shape[0]}] with a contiguous last dim")
-    if tuple(rows.shape) != (m,) or not rows.is_contiguous():
+    if rows.shape != (m,) or not rows.is_contiguous():
         raise H3Error(f"rows must be a contiguous int32 [{m}]")
     rank = lora_a.shape[0] // n_adapters
     with _on(dev):
-        ws_bytes = _adapters_workspace(dev.index, m, chunks, chunk_cols, n, ep, rank, n_adapters)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        ws_bytes = _adapters_workspace(dev, m, chunks, chunk_cols, n, ep, rank, n_adapters)
+        ws = a.new_empty(((ws_bytes + 1) // 2,))
         rc = lib().h3_gemm_adapters(a.data_ptr(), m, chunks, chunk_cols, chunk_stride, row_stride, weight.data_ptr(), n,
                                     weight.stride(0), lora_a.data_ptr(), lora_a.stride(0), lora_b.data_ptr(),
                                     lora_b.stride(0), rank, n_adapters, scale.data_ptr(), rows.data_ptr(),
                                     out.data_ptr(), out.stride(0), ep, ws.data_ptr(), ws_bytes,
-                                    status_word(dev).data_ptr(), _stream())
+                                    _status_ptr(dev), _stream())
     _check(rc, "h3_gemm_adapters")
     return out
 

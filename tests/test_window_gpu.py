@@ -76,6 +76,26 @@ def test_against_the_definition(cuda_dev, case):
     _check(o, ref, mag)
 
 
+# more blocks of queries than the GPU holds CTAs: (heads, key heads, queries, keys, left, right, sinks, causal, q_start)
+MANY = [(40, 40, 1500, 1500, 70, 30, 20, False, 0), (48, 24, 1000, 1000, None, 0, 0, True, 0),
+        (300, 300, 130, 600, 100, 0, 200, True, 470), (64, 64, 900, 400, 10, 10, 0, False, -450),
+        (64, 64, 900, 300, 40, 0, 7, True, 0), (400, 400, 20, 500, 120, 5, 30, False, 200),
+        (600, 300, 50, 350, 3, 0, 0, True, 320), (350, 350, 9, 200, 1, 1, 0, False, 150)]
+
+
+@pytest.mark.parametrize("case", MANY, ids=str)
+@pytest.mark.parametrize("splits", [None, 1])
+def test_more_blocks_than_ctas(cuda_dev, case, splits):
+    import h3attn as O
+    H, hk, sq, skv, left, right, sinks, causal, q_start = case
+    q, k, v = _rand((H, sq, D), 1, cuda_dev), _rand((hk, skv, D), 2, cuda_dev), _rand((hk, skv, D), 3, cuda_dev)
+    out = torch.full((H, sq, D), 9.0, dtype=torch.bfloat16, device=cuda_dev)
+    o, (ref, mag) = _run(O, q, k, v, left, right, sinks, causal, q_start, out=out, splits=splits)
+    _check(o, ref, mag)
+    assert torch.equal(o, O.window_attention(q, k, v, left, right, sinks=sinks, causal=causal, q_start=q_start,
+                                             splits=splits))
+
+
 @pytest.mark.parametrize("splits", [1, 2, 3, 7, 64])
 def test_any_number_of_splits(cuda_dev, splits):
     import h3attn as O
