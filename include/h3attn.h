@@ -177,12 +177,12 @@ int h3_attn_fwd_peer(const void* q, const void* k, const void* v, void* o_local,
  *   q: [n_heads][s_q][128], k, v: [n_kv_heads][s_kv][128] (strides as h3_attn_fwd; n_heads a multiple of n_kv_heads,
  *   at most 128 times it; query head h reads key head h / (n_heads / n_kv_heads)); o as h3_attn_fwd. Lengths and
  *   |q_start| up to 2^29.
- * h3_window_attn_plan returns the number of splits of the key axis (>= 1, or an error) that h3_window_attn should be
- * given, and the bytes of fp32 workspace (16-byte aligned, 0 for one split) that it then needs; splits = 0 lets the
- * plan choose by the call's shape and the GPU, 1..64 fixes it. One split gives every query row the same bits whatever
- * heads share the call. The workspace may be reused once the call's work on the stream is done. */
-int h3_window_attn_plan(int64_t n_heads, int64_t n_kv_heads, int64_t s_q, int64_t s_kv, int64_t left, int64_t right,
-                        int64_t sinks, int32_t causal, int64_t q_start, int64_t splits, int64_t* ws_bytes);
+ * splits: how many parts the key axis of a block of queries is worked in: 0 lets the call choose by its shape and the
+ * GPU, 1 splits nothing (a query row's bits then do not depend on which heads share the call), up to 64.
+ * h3_window_attn_workspace returns the bytes of fp32 workspace that a call needs (16-byte aligned; 0: none), or an
+ * error; it may be reused once the call's work on the stream is done. */
+int64_t h3_window_attn_workspace(int64_t n_heads, int64_t n_kv_heads, int64_t s_q, int64_t s_kv, int64_t left,
+                                 int64_t right, int64_t sinks, int32_t causal, int64_t q_start, int64_t splits);
 int h3_window_attn(const void* q, const void* k, const void* v, void* o, int64_t n_heads, int64_t n_kv_heads,
                    int64_t s_q, int64_t s_kv, int64_t q_head_stride, int64_t q_row_stride, int64_t kv_head_stride,
                    int64_t kv_row_stride, int64_t o_rank_rows, int64_t o_rank_stride, int64_t o_head_stride,

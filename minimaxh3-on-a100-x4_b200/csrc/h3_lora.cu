@@ -448,8 +448,9 @@ __global__ void __launch_bounds__(192, 2)
   }
 }
 
-// Two neighbouring columns a thread, kFinishRows rows a CTA: the pieces of W x in ascending order, plus B_a T.
-constexpr int kFinishRows = 4;
+// One row and 256 columns a CTA, two neighbouring columns a thread: the pieces of W x in ascending order, plus B_a T.
+// The first kAhead * 8 columns of B are loaded before the wait for stream_kernel (they do not depend on it).
+constexpr int kAhead = 4;
 
 struct Finish {
   const __nv_bfloat16* b;  // stacked B
@@ -459,72 +460,98 @@ struct Finish {
   int n_out, swiglu;
 };
 
-__device__ __forceinline__ float2 finish_pair(const Stream& s, const Finish& f, const float* t, int rank, int col0,
-                                              int row, int n) {
-  const int tile = n / 128, pieces = pieces_of(s, tile);
-  float2 y = make_float2(0.f, 0.f);
-  for (int q = 0; q < pieces; ++q) {
-    const float2 v = *reinterpret_cast<const float2*>(s.part + ((long long)q * s.m + row) * s.columns + n);
-    y.x += v.x;
-    y.y += v.y;
-  }
-  if (col0 >= 0) {
-    float2 d = make_float2(0.f, 0.f);
-    const __nv_bfloat16* b0 = f.b + n * f.b_row + col0;
-    const __nv_bfloat16* b1 = b0 + f.b_row;
-    for (int j = 0; j < rank; j += 8) {
-      float w0[8], w1[8];
-      bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(b0 + j)), w0);
-      bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(b1 + j)), w1);
+// Columns n and n + 1 of a row.
+struct FinishPair {
+  uint4 b0[kAhead], b1[kAhead];
+  const __nv_bfloat16* from;
+
+  __device__ __forceinline__ void load(const Finish& f, int col0, int rank, int n) {
+    from = f.b + n * f.b_row + col0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        d.x += w0[e] * t[j + e];
-        d.y += w1[e] * t[j + e];
+    for (int q = 0; q < kAhead; ++q)
+      if (col0 >= 0 && 8 * q < rank) {
+        b0[q] = __ldg(reinterpret_cast<const uint4*>(from + 8 * q));
+        b1[q] = __ldg(reinterpret_cast<const uint4*>(from + f.b_row + 8 * q));
       }
-    }
-    y.x += d.x;
-    y.y += d.y;
   }
-  return y;
-}
+  __device__ __forceinline__ float2 pieces(const Stream& s, int row, int n) const {
+    const int count = pieces_of(s, n / 128);
+    const float* at = s.part + row * s.columns + n;
+    float2 y = make_float2(0.f, 0.f);
+#pragma unroll 4
+    for (int q = 0; q < count; ++q) {
+      const float2 v = *reinterpret_cast<const float2*>(at + (long long)q * s.m * s.columns);
+      y.x += v.x;
+      y.y += v.y;
+    }
+    return y;
+  }
+  static __device__ __forceinline__ void dot8(const uint4& u0, const uint4& u1, const float* t, float2& d) {
+    float w0[8], w1[8];
+    bf16x8_to_f32(u0, w0);
+    bf16x8_to_f32(u1, w1);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      d.x += w0[e] * t[e];
+      d.y += w1[e] * t[e];
+    }
+  }
+  __device__ __forceinline__ float2 low(const Finish& f, const float* t, int rank) const {
+    float2 d = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q)
+      if (8 * q < rank) dot8(b0[q], b1[q], t + 8 * q, d);
+    for (int j = 8 * kAhead; j < rank; j += 8)
+      dot8(__ldg(reinterpret_cast<const uint4*>(from + j)), __ldg(reinterpret_cast<const uint4*>(from + f.b_row + j)),
+           t + j, d);
+    return d;
+  }
+};
 
 __global__ void __launch_bounds__(128) finish_kernel(const Adapters ad, const Stream s, const Finish f) {
-  __shared__ float t[kFinishRows][kMaxRank];
-  __shared__ int first[kFinishRows];
+  __shared__ float t[kMaxRank];
+  const int row = blockIdx.y;
+  const int a = adapter_of(ad, s.m, row);
+  const int col0 = a < 0 ? -1 : a * ad.rank;
+  const int n = blockIdx.x * 256 + 2 * threadIdx.x;
+  const bool mine = n < f.n_out;
+  FinishPair y, u;
+  if (mine) y.load(f, col0, ad.rank, n);
+  if (mine && f.swiglu) u.load(f, col0, ad.rank, f.n_out + n);
   pdl_wait();
   if (*reinterpret_cast<volatile int*>(s.status) != 0) return;
-  const int r0 = blockIdx.y * kFinishRows;
-  if (threadIdx.x < kFinishRows) {
-    const int a = adapter_of(ad, s.m, r0 + threadIdx.x);
-    first[threadIdx.x] = a < 0 ? -1 : a * ad.rank;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < kFinishRows * ad.rank; i += 128) {
-    const int r = i / ad.rank, j = i - r * ad.rank;
-    if (first[r] < 0) continue;
-    const int col = 128 * s.w_tiles + first[r] + j;
-    const int pieces = pieces_of(s, col / 128);
-    float v = 0.f;
-    for (int q = 0; q < pieces; ++q) v += s.part[((long long)q * s.m + r0 + r) * s.columns + col];
-    t[r][j] = v * ad.scale[first[r] / ad.rank];
-  }
-  __syncthreads();
-  const int n = blockIdx.x * 256 + 2 * threadIdx.x;
-  if (n >= f.n_out) return;
-#pragma unroll
-  for (int r = 0; r < kFinishRows; ++r) {
-    const int row = r0 + r;
-    if (row >= s.m) break;
-    float2 y = finish_pair(s, f, t[r], ad.rank, first[r], row, n);
-    if (f.swiglu) {
-      // out = bf16(bf16(silu(g)) * u), g and u the bf16-rounded gate / up projections
-      const float2 u = finish_pair(s, f, t[r], ad.rank, first[r], row, f.n_out + n);
-      const float g0 = bf16_round(y.x), g1 = bf16_round(y.y);
-      y.x = bf16_round(g0 / (1.0f + __expf(-g0))) * bf16_round(u.x);
-      y.y = bf16_round(g1 / (1.0f + __expf(-g1))) * bf16_round(u.y);
+  if (a >= 0) {
+    for (int j = threadIdx.x; j < ad.rank; j += 128) {
+      const int col = 128 * s.w_tiles + col0 + j;
+      const int count = pieces_of(s, col / 128);
+      float v = 0.f;
+#pragma unroll 4
+      for (int q = 0; q < count; ++q) v += s.part[((long long)q * s.m + row) * s.columns + col];
+      t[j] = v * ad.scale[a];
     }
-    *reinterpret_cast<uint32_t*>(f.c + (long long)row * f.ldc + n) = pack_bf16x2(y.x, y.y);
   }
+  float2 gy = make_float2(0.f, 0.f), gu = gy;
+  if (mine) gy = y.pieces(s, row, n);
+  if (mine && f.swiglu) gu = u.pieces(s, row, f.n_out + n);
+  __syncthreads();
+  if (!mine) return;
+  if (a >= 0) {
+    const float2 d = y.low(f, t, ad.rank);
+    gy.x += d.x;
+    gy.y += d.y;
+  }
+  if (f.swiglu) {
+    if (a >= 0) {
+      const float2 d = u.low(f, t, ad.rank);
+      gu.x += d.x;
+      gu.y += d.y;
+    }
+    // out = bf16(bf16(silu(g)) * u), g and u the bf16-rounded gate / up projections
+    const float g0 = bf16_round(gy.x), g1 = bf16_round(gy.y);
+    gy.x = bf16_round(g0 / (1.0f + __expf(-g0))) * bf16_round(gu.x);
+    gy.y = bf16_round(g1 / (1.0f + __expf(-g1))) * bf16_round(gu.y);
+  }
+  *reinterpret_cast<uint32_t*>(f.c + (long long)row * f.ldc + n) = pack_bf16x2(gy.x, gy.y);
 }
 
 // ---------------------------------------------------------------- host
@@ -636,7 +663,7 @@ extern "C" int h3_gemm_adapters(const void* a, int64_t m, int64_t a_chunks, int6
     if (cudaGetLastError() != cudaSuccess) return H3_ERR_LAUNCH;
     const Finish f = {reinterpret_cast<const __nv_bfloat16*>(lora_b), lora_b_row_stride,
                       reinterpret_cast<__nv_bfloat16*>(c), c_row_stride, (int)n_out, epilogue};
-    const dim3 grid((unsigned)((n_out + 255) / 256), (unsigned)((m + kFinishRows - 1) / kFinishRows));
+    const dim3 grid((unsigned)((n_out + 255) / 256), (unsigned)m);
     return launch_dependent(finish_kernel, grid, 128, 0, st, ad, l.s, f);
   }
   if ((rc = map_a(&tx, call)) != H3_OK) return rc;

@@ -21,7 +21,7 @@
 // kTiles = 2: CTA = 256 packed rows, 12 warps, 5-stage K/V ring, one CTA per SM (the full kernel's
 // schedule). kTiles = 1: CTA = 128 packed rows, 8 warps, 2-stage ring, two CTAs per SM. Few rows split the tile
 // list over gridDim.z CTAs; each writes (O, m, l) in fp32 to the caller's workspace and join_kernel
-// combines them in a fixed order.
+// combines them in a fixed order. A single token has a kernel of its own (token_kernel).
 #include <algorithm>
 #include <cmath>
 
@@ -103,6 +103,7 @@ __global__ void __launch_bounds__(Cfg<kTiles>::kThreads, Cfg<kTiles>::kCtasPerSm
     window_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                   const __grid_constant__ CUtensorMap tmap_v, const Params p) {
   using C = Cfg<kTiles>;
+  pdl_launch_dependents();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
@@ -463,12 +464,18 @@ __global__ void __launch_bounds__(Cfg<kTiles>::kThreads, Cfg<kTiles>::kCtasPerSm
   }
 }
 
-// One warp per output row: the splits' (O, m, l) joined in ascending order, normalised and rounded once.
-__global__ void __launch_bounds__(128) join_kernel(const Params p, int splits) {
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
+// One CTA per output row: its warps take the splits' (O, m, l) in turn, all loads in flight at once; the sums are
+// joined in a fixed order, normalised and rounded once.
+constexpr int kJoinWarps = 8;
+
+__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Params p, int splits) {
+  __shared__ float4 sh_o[kJoinWarps][32];
+  __shared__ float sh_l[kJoinWarps];
+  pdl_wait();
+  if (*reinterpret_cast<volatile int*>(p.status) != 0) return;
+  const long long row = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long rows = (long long)p.n_heads * p.s_q;
-  if (row >= rows || *reinterpret_cast<volatile int*>(p.status) != 0) return;
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
   float m = -INFINITY;
   for (int s = lane; s < splits; s += 32) m = fmaxf(m, ml[s * rows + row].x);
@@ -478,7 +485,7 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p, int splits) {
   float l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int s = 0; s < splits; ++s) {
+  for (int s = warp; s < splits; s += kJoinWarps) {
     const float2 v = ml[s * rows + row];
     const float4 o = reinterpret_cast<const float4*>(p.part_o + (s * rows + row) * 128)[lane];
     const float f = ex2_approx(v.x - m_use);
@@ -488,12 +495,185 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p, int splits) {
     acc.z += f * o.z;
     acc.w += f * o.w;
   }
+  sh_o[warp][lane] = acc;
+  if (lane == 0) sh_l[warp] = l;
+  __syncthreads();
+  if (warp != 0) return;
+#pragma unroll
+  for (int w = 1; w < kJoinWarps; ++w) {
+    const float4 o = sh_o[w][lane];
+    l += sh_l[w];
+    acc.x += o.x;
+    acc.y += o.y;
+    acc.z += o.z;
+    acc.w += o.w;
+  }
   const float inv = l == 0.f ? 0.f : 1.0f / l;
   const long long i = row % p.s_q, head = row / p.s_q;
   __nv_bfloat16* dst = p.o + (i / p.o_rank_rows) * p.o_rank_stride + head * p.o_head_stride +
                        (i % p.o_rank_rows) * p.o_row_stride;
   reinterpret_cast<uint2*>(dst)[lane] =
       make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+}
+
+// ---------------------------------------------------------------- single tokens
+// One query position and kGroup query heads to a key head (at most 4): every key of the walk is visible to every row,
+// so there is nothing to mask, and a 128-row tile would be all padding. A cluster of CTAs takes the keys of one
+// key head, one run of them each; a half-warp takes a key (16 bytes of K and of V a lane), kKeys keys at a time in
+// flight, with its own running maximum and sums; half-warps join through shared memory, CTAs through distributed
+// shared memory. One launch, no workspace, and bound by the loads: 16 B x 2 x kKeys x 256 lanes a CTA in flight.
+constexpr int kTokenWarps = 8;
+constexpr int kKeys = 4;  // keys in flight per half-warp
+constexpr int kTokenMaxCluster = 8;
+
+struct TokenParams {
+  const __nv_bfloat16 *q, *k, *v;
+  long long q_head, kv_head, kv_row;
+};
+
+template <int kGroup>
+__global__ void __launch_bounds__(32 * kTokenWarps) token_kernel(const Params p, const TokenParams tp) {
+  constexpr int kHalves = 2 * kTokenWarps;
+  __shared__ float sh_m[kHalves][kGroup], sh_l[kHalves][kGroup];
+  __shared__ float sh_o[kHalves][kGroup][kHeadDim];
+  __shared__ float cta_m[kGroup], cta_l[kGroup], cta_o[kGroup][kHeadDim];
+  const int lane = threadIdx.x & 31, sub = lane & 15;
+  const int half = threadIdx.x >> 4;
+  const int rank = int(cluster_ctarank()), ranks = int(gridDim.x);
+  const int kvh = blockIdx.y;
+  const bool live = *reinterpret_cast<volatile int*>(p.status) == 0;
+  const Walk walk = make_walk(p, p.q_start, p.q_start);
+  const bool window = walk.n > walk.a_tiles;
+  const int n_first = walk.a_tiles > 0 ? walk.a_end : 0;  // keys of the separate first-token run
+  const int total = live ? n_first + (window ? walk.b_end - walk.b_start : 0) : 0;
+  const int k0 = int((long long)total * rank / ranks), k1 = int((long long)total * (rank + 1) / ranks);
+  const __nv_bfloat16* kb = tp.k + kvh * tp.kv_head + 8 * sub;
+  const __nv_bfloat16* vb = tp.v + kvh * tp.kv_head + 8 * sub;
+
+  float q[kGroup][8], acc[kGroup][8], m[kGroup], l[kGroup];
+#pragma unroll
+  for (int g = 0; g < kGroup; ++g) {
+    bf16x8_to_f32(*reinterpret_cast<const uint4*>(tp.q + (long long)(kvh * kGroup + g) * tp.q_head + 8 * sub), q[g]);
+    m[g] = -INFINITY;
+    l[g] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      q[g][e] *= p.scale_log2;
+      acc[g][e] = 0.f;
+    }
+  }
+  for (int base = k0 + half * kKeys; base < k1; base += kHalves * kKeys) {
+    uint4 ku[kKeys], vu[kKeys];
+    bool in[kKeys];
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) {
+      in[i] = base + i < k1;
+      const int at = in[i] ? base + i : base;
+      const long long key = at < n_first ? at : walk.b_start + (at - n_first);
+      ku[i] = __ldg(reinterpret_cast<const uint4*>(kb + key * tp.kv_row));
+      vu[i] = __ldg(reinterpret_cast<const uint4*>(vb + key * tp.kv_row));
+    }
+    float s[kGroup][kKeys];
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) {
+      float kf[8];
+      bf16x8_to_f32(ku[i], kf);
+#pragma unroll
+      for (int g = 0; g < kGroup; ++g) {
+        float d = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) d += q[g][e] * kf[e];
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) d += __shfl_xor_sync(half & 1 ? 0xffff0000u : 0x0000ffffu, d, o);
+        s[g][i] = in[i] ? d : -INFINITY;
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < kGroup; ++g) {
+      float top = m[g];
+#pragma unroll
+      for (int i = 0; i < kKeys; ++i) top = fmaxf(top, s[g][i]);
+      const float use = top == -INFINITY ? 0.f : top;
+      const float f = ex2_approx(m[g] - use);
+      m[g] = top;
+      l[g] *= f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[g][e] *= f;
+#pragma unroll
+      for (int i = 0; i < kKeys; ++i) {
+        s[g][i] = ex2_approx(s[g][i] - use);
+        l[g] += s[g][i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) {
+      float vf[8];
+      bf16x8_to_f32(vu[i], vf);
+      if (in[i]) {  // a key past the share is not added, whatever its V holds
+#pragma unroll
+        for (int g = 0; g < kGroup; ++g)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[g][e] += s[g][i] * vf[e];
+      }
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < kGroup; ++g) {
+    if (sub == 0) {
+      sh_m[half][g] = m[g];
+      sh_l[half][g] = l[g];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sh_o[half][g][8 * sub + e] = acc[g][e];
+  }
+  __syncthreads();
+  // the CTA's half-warps, in ascending order
+  for (int t = threadIdx.x; t < kGroup * kHeadDim; t += 32 * kTokenWarps) {
+    const int g = t / kHeadDim, d = t % kHeadDim;
+    float top = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) top = fmaxf(top, sh_m[h][g]);
+    const float use = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, o = 0.f;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+      const float f = ex2_approx(sh_m[h][g] - use);
+      sum += f * sh_l[h][g];
+      o += f * sh_o[h][g][d];
+    }
+    cta_o[g][d] = o;
+    if (d == 0) {
+      cta_m[g] = top;
+      cta_l[g] = sum;
+    }
+  }
+  cluster_sync_all();
+  // the cluster's CTAs, in ascending order: each finishes its share of the outputs, two neighbouring elements a thread
+  const int pairs = kGroup * kHeadDim / 2;
+  for (int t = rank * 32 * kTokenWarps + threadIdx.x; live && t < pairs; t += ranks * 32 * kTokenWarps) {
+    const int g = 2 * t / kHeadDim, d = 2 * t % kHeadDim;
+    float pm[kTokenMaxCluster], top = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < kTokenMaxCluster; ++r) {
+      pm[r] = r < ranks ? ld_cluster_f32(mapa_shared(smem_u32(&cta_m[g]), r)) : -INFINITY;
+      top = fmaxf(top, pm[r]);
+    }
+    const float use = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+    for (int r = 0; r < kTokenMaxCluster; ++r) {
+      if (r < ranks) {
+        const float f = ex2_approx(pm[r] - use);
+        sum += f * ld_cluster_f32(mapa_shared(smem_u32(&cta_l[g]), r));
+        o0 += f * ld_cluster_f32(mapa_shared(smem_u32(&cta_o[g][d]), r));
+        o1 += f * ld_cluster_f32(mapa_shared(smem_u32(&cta_o[g][d + 1]), r));
+      }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+    *reinterpret_cast<uint32_t*>(p.o + (long long)(kvh * kGroup + g) * p.o_head_stride + d) =
+        pack_bf16x2(o0 * inv, o1 * inv);
+  }
+  cluster_sync_all();  // no CTA leaves while another reads its shared memory
 }
 
 // ---------------------------------------------------------------- host
@@ -519,11 +699,13 @@ struct Plan {
   int tile_pos; // query positions per Q tile
   unsigned grid_x;
   int splits;
+  int token;     // cluster size of token_kernel, or 0: window_kernel
 };
 
-// Q tiles per CTA: two (256 packed rows, one CTA an SM) where the rows fill them, else one (two CTAs an SM).
-// Splits: only when the unsplit grid leaves CTA slots empty; then as many as fill them, with at least two
-// key tiles each.
+// A single token with at most 4 query heads to a key head, and key heads enough that clusters of 8 CTAs reach most SMs:
+// token_kernel, a CTA for 128 keys up to 8 of them. Else Q tiles of window_kernel: two per CTA (256 packed rows, one
+// CTA an SM) where the rows fill more than one, else one (two CTAs an SM); and splits only when the unsplit grid
+// leaves CTA slots empty: then as many as fill them, with at least two key tiles each.
 static int make_plan(const Shape& s, int64_t splits_asked, Plan& pl) {
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
@@ -537,9 +719,15 @@ static int make_plan(const Shape& s, int64_t splits_asked, Plan& pl) {
   const int64_t left = s.left < 0 || s.left > kMaxPos ? kMaxPos : s.left;
   const int64_t right = s.causal ? 0 : (s.right < 0 || s.right > kMaxPos ? kMaxPos : s.right);
   const int64_t span = std::min(s.s_kv, left + right + per_cta) + std::min(s.sinks, s.s_kv);
-  const int64_t tiles = (std::min(span, s.s_kv) + kBlockN - 1) / kBlockN;
+  const int64_t key_tiles = (std::min(span, s.s_kv) + kBlockN - 1) / kBlockN;
+  pl.token = 0;
+  if (splits_asked == 0 && s.s_q == 1 && group <= 4 && s.n_kv_heads * kTokenMaxCluster >= sms) {
+    pl.token = (int)std::max<int64_t>(1, std::min<int64_t>(kTokenMaxCluster, key_tiles));
+    pl.splits = 1;
+    return H3_OK;
+  }
   int64_t splits = splits_asked;
-  if (splits == 0) splits = std::min(slots / std::max<int64_t>(ctas, 1), tiles / 2);
+  if (splits == 0) splits = std::min(slots / std::max<int64_t>(ctas, 1), key_tiles / 2);
   pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits));
   return H3_OK;
 }
@@ -588,18 +776,16 @@ static int launch(cudaStream_t st, const CUtensorMap& q, const CUtensorMap& k, c
 using namespace h3;
 using namespace h3::window;
 
-extern "C" int h3_window_attn_plan(int64_t n_heads, int64_t n_kv_heads, int64_t s_q, int64_t s_kv, int64_t left,
-                                   int64_t right, int64_t sinks, int32_t causal, int64_t q_start, int64_t splits,
-                                   int64_t* ws_bytes) {
-  if (!ws_bytes) return H3_ERR_NULL;
+extern "C" int64_t h3_window_attn_workspace(int64_t n_heads, int64_t n_kv_heads, int64_t s_q, int64_t s_kv,
+                                            int64_t left, int64_t right, int64_t sinks, int32_t causal,
+                                            int64_t q_start, int64_t splits) {
   const Shape s = {n_heads, n_kv_heads, s_q, s_kv, left, right, sinks, q_start, causal};
   int rc;
   if ((rc = check_shape(s)) != H3_OK) return rc;
   if (splits < 0 || splits > kMaxSplits) return H3_ERR_SHAPE;
   Plan pl;
   if ((rc = make_plan(s, splits, pl)) != H3_OK) return rc;
-  *ws_bytes = workspace_bytes(s, pl);
-  return pl.splits;
+  return workspace_bytes(s, pl);
 }
 
 extern "C" int h3_window_attn(const void* q, const void* k, const void* v, void* o, int64_t n_heads,
@@ -615,7 +801,7 @@ extern "C" int h3_window_attn(const void* q, const void* k, const void* v, void*
   const Shape s = {n_heads, n_kv_heads, s_q, s_kv, left, right, sinks, q_start, causal};
   int rc;
   if ((rc = check_shape(s)) != H3_OK) return rc;
-  if (o_rank_rows < 1 || splits < 1 || splits > kMaxSplits) return H3_ERR_SHAPE;
+  if (o_rank_rows < 1 || splits < 0 || splits > kMaxSplits) return H3_ERR_SHAPE;
   if (!(softmax_scale > 0.f) || !std::isfinite(softmax_scale)) return H3_ERR_SHAPE;
   if (q_row_stride < 128 || kv_row_stride < 128 || o_row_stride < 128 || (q_row_stride % 8) || (kv_row_stride % 8) ||
       (q_head_stride % 8) || (kv_head_stride % 8) || (o_row_stride % 8) || (o_head_stride % 8) ||
@@ -624,14 +810,8 @@ extern "C" int h3_window_attn(const void* q, const void* k, const void* v, void*
     return H3_ERR_STRIDE;
   Plan pl;
   if ((rc = make_plan(s, splits, pl)) != H3_OK) return rc;
-  if (pl.splits > 1 && !workspace) return H3_ERR_NULL;
   if (ws_bytes < workspace_bytes(s, pl)) return H3_ERR_WORKSPACE;
-
-  CUtensorMap mq, mk, mv;
-  const long long kvhs = n_kv_heads > 1 ? kv_head_stride : s_kv * kv_row_stride;
-  if ((rc = make_q_map(&mq, q, s, q_head_stride, q_row_stride, pl.tile_pos)) != H3_OK) return rc;
-  if ((rc = make_head_map(&mk, k, s_kv, n_kv_heads, kv_row_stride, kvhs)) != H3_OK) return rc;
-  if ((rc = make_head_map(&mv, v, s_kv, n_kv_heads, kv_row_stride, kvhs)) != H3_OK) return rc;
+  if (pl.splits > 1 && !workspace) return H3_ERR_NULL;
 
   Params p;
   p.n_heads = (int)n_heads;
@@ -654,9 +834,32 @@ extern "C" int h3_window_attn(const void* q, const void* k, const void* v, void*
   p.part_ml = pl.splits > 1 ? p.part_o + (int64_t)pl.splits * n_heads * s_q * 128 : nullptr;
   p.status = status;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (pl.token > 0) {
+    const TokenParams tp = {reinterpret_cast<const __nv_bfloat16*>(q), reinterpret_cast<const __nv_bfloat16*>(k),
+                            reinterpret_cast<const __nv_bfloat16*>(v), q_head_stride, kv_head_stride, kv_row_stride};
+    auto* kern = p.group == 1 ? token_kernel<1> : p.group == 2 ? token_kernel<2> : p.group == 3 ? token_kernel<3>
+                                                                                               : token_kernel<4>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)pl.token, (unsigned)n_kv_heads);
+    cfg.blockDim = dim3(32 * kTokenWarps);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)pl.token;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, kern, p, tp) != cudaSuccess) return H3_ERR_LAUNCH;
+    return cudaGetLastError() == cudaSuccess ? H3_OK : H3_ERR_LAUNCH;
+  }
+  CUtensorMap mq, mk, mv;
+  const long long kvhs = n_kv_heads > 1 ? kv_head_stride : s_kv * kv_row_stride;
+  if ((rc = make_q_map(&mq, q, s, q_head_stride, q_row_stride, pl.tile_pos)) != H3_OK) return rc;
+  if ((rc = make_head_map(&mk, k, s_kv, n_kv_heads, kv_row_stride, kvhs)) != H3_OK) return rc;
+  if ((rc = make_head_map(&mv, v, s_kv, n_kv_heads, kv_row_stride, kvhs)) != H3_OK) return rc;
   rc = pl.tiles == 2 ? launch<2>(st, mq, mk, mv, p, pl, (unsigned)n_kv_heads)
                      : launch<1>(st, mq, mk, mv, p, pl, (unsigned)n_kv_heads);
   if (rc != H3_OK || pl.splits == 1) return rc;
-  join_kernel<<<(unsigned)((n_heads * s_q + 3) / 4), 128, 0, st>>>(p, pl.splits);
-  return cudaGetLastError() == cudaSuccess ? H3_OK : H3_ERR_LAUNCH;
+  return launch_dependent(join_kernel, dim3((unsigned)(n_heads * s_q)), 32 * kJoinWarps, 0, st, p, pl.splits);
 }

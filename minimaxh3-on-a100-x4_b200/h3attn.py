@@ -102,8 +102,8 @@ def lib() -> ctypes.CDLL:
         L.h3_qknorm_rope_pack_peer.restype = ctypes.c_int
         L.h3_attn_fwd_peer.argtypes = [vp] * 5 + [i64] * 11 + [ctypes.c_float, i32p, vp]
         L.h3_attn_fwd_peer.restype = ctypes.c_int
-        L.h3_window_attn_plan.argtypes = [i64] * 7 + [ctypes.c_int32, i64, i64, vp]
-        L.h3_window_attn_plan.restype = ctypes.c_int
+        L.h3_window_attn_workspace.argtypes = [i64] * 7 + [ctypes.c_int32, i64, i64]
+        L.h3_window_attn_workspace.restype = i64
         L.h3_window_attn.argtypes = [vp] * 4 + [i64] * 12 + [f32, i64, i64, i64, ctypes.c_int32, i64, i64, vp, i64, i32p,
                                      vp]
         L.h3_window_attn.restype = ctypes.c_int
@@ -243,14 +243,12 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, s_kv: int | Non
 
 # ----------------------------------------------------------------------------- windowed attention
 @functools.lru_cache(maxsize=4096)
-def _window_plan(dev_index: int, *shape) -> tuple:
-    """(splits, workspace bytes) of a windowed attention call on the current device; a pure function of
-    its sizes."""
-    n = ctypes.c_int64()
-    rc = lib().h3_window_attn_plan(*shape, ctypes.byref(n))
-    if rc < 0:
-        _check(rc, "h3_window_attn_plan")
-    return rc, n.value
+def _window_workspace(dev_index: int, *shape) -> int:
+    """Workspace bytes of a windowed attention call of these sizes on the current device."""
+    n = lib().h3_window_attn_workspace(*shape)
+    if n < 0:
+        _check(n, "h3_window_attn_workspace")
+    return n
 
 
 def _head_strides(t: torch.Tensor, heads: int, rows: int) -> tuple:
@@ -306,11 +304,11 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: in
     lo, hi = (-1 if side is None or side > big else int(side) for side in (left, right))
     sinks = min(int(sinks), s_kv)
     with _on(dev):
-        n_splits, ws_bytes = _window_plan(dev, H, hk, sq, s_kv, lo, hi, sinks, int(causal), q_start, splits or 0)
+        ws_bytes = _window_workspace(dev, H, hk, sq, s_kv, lo, hi, sinks, int(causal), q_start, splits or 0)
         ws = q.new_empty((ws_bytes // 2,)) if ws_bytes else None
         rc = lib().h3_window_attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), H, hk, sq, s_kv,
                                   *q_st, *k_st, rank_rows, rank_stride,
-                                  head_stride, row_stride, scale, lo, hi, sinks, int(causal), q_start, n_splits,
+                                  head_stride, row_stride, scale, lo, hi, sinks, int(causal), q_start, splits or 0,
                                   ws.data_ptr() if ws_bytes else None, ws_bytes, _status_ptr(dev), _stream())
     _check(rc, "h3_window_attn")
     return out

@@ -71,7 +71,7 @@ def test_window_rejects_bad_arguments_before_launch(L):
           100, 0, 4, 1, 436, 1, None, 0, st, None]  # left right sinks causal q_start splits ws bytes status stream
     for at, value, code in ((0, None, -1), (25, None, -1), (3, ctypes.c_void_p(0x1008), -2), (4, 9, -3), (5, 0, -3),
                             (6, 0, -3), (7, 0, -3), (7, (1 << 29) + 1, -3), (19, -1, -3), (21, 1 << 30, -3),
-                            (22, 0, -3), (22, 65, -3), (12, 0, -3), (16, ctypes.c_float(0.0), -3),
+                            (22, -1, -3), (22, 65, -3), (12, 0, -3), (16, ctypes.c_float(0.0), -3),
                             (16, ctypes.c_float(float("nan")), -3), (9, 100, -4), (9, 120, -4), (11, 64, -4),
                             (8, 0, -4), (10, 0, -4), (15, 64, -4), (14, -8, -4)):
         bad = list(ok)
@@ -80,10 +80,8 @@ def test_window_rejects_bad_arguments_before_launch(L):
     bad = list(ok)
     bad[4], bad[5] = 258, 2  # more than 128 query heads to a key head
     assert L.h3_window_attn(*bad) == -3
-    assert L.h3_window_attn_plan(8, 2, 64, 500, 100, 0, 4, 1, 436, 0, None) == -1
-    n = ctypes.c_int64()
-    assert L.h3_window_attn_plan(8, 3, 64, 500, 100, 0, 4, 1, 436, 0, ctypes.byref(n)) == -3
-    assert L.h3_window_attn_plan(8, 2, 64, 500, 100, 0, 4, 1, 436, 65, ctypes.byref(n)) == -3
+    assert L.h3_window_attn_workspace(8, 3, 64, 500, 100, 0, 4, 1, 436, 0) == -3
+    assert L.h3_window_attn_workspace(8, 2, 64, 500, 100, 0, 4, 1, 436, 65) == -3
 
 
 def _walk(left, right, sinks, causal, s_kv, p_first, p_last, tile=128):

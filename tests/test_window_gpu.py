@@ -96,6 +96,31 @@ def test_more_blocks_than_ctas(cuda_dev, case, splits):
                                              splits=splits))
 
 
+@pytest.mark.parametrize("H,hk", [(20, 20), (40, 20), (57, 19), (80, 20), (100, 20)])
+@pytest.mark.parametrize("skv,left,right,sinks,q_start", [
+    (1, 0, 0, 0, 0), (2, 0, 0, 1, 1), (63, None, 0, 0, 62), (64, 10, 0, 5, 63), (129, None, None, 0, 60),
+    (1000, 300, 0, 100, 999), (1000, 300, 20, 700, 800), (5000, 4097, 0, 3, 4999), (777, 5, 5, 0, 5000),
+    (777, 5, 5, 9, 5000), (777, 40, 0, 0, -3)])
+def test_single_tokens(cuda_dev, H, hk, skv, left, right, sinks, q_start):
+    """One query position over a cache: groups of 1 to 4 query heads to a key head have a kernel of their own, 5 go
+    through the tiles; one, two or no runs of keys, and NaN wherever the token does not look."""
+    import h3attn as O
+    q, k, v = _rand((H, 1, D), 1, cuda_dev), _rand((hk, skv + 9, D), 2, cuda_dev), _rand((hk, skv + 9, D), 3, cuda_dev)
+    j = torch.arange(skv + 9, device=cuda_dev)
+    seen = (j < sinks) | ((j >= q_start - (left if left is not None else 10 ** 6)) &
+                          (j <= q_start + (right if right is not None else 10 ** 6)))
+    k[:, ~seen | (j >= skv)] = float("nan")
+    v[:, ~seen | (j >= skv)] = float("inf")
+    out = torch.full((H, 1, D), 5.0, dtype=torch.bfloat16, device=cuda_dev)
+    o = O.window_attention(q, k, v, left, right, sinks=sinks, q_start=q_start, s_kv=skv, out=out)
+    O.check_status()
+    k, v = (torch.where(seen[None, :, None], t, torch.zeros_like(t)) for t in (k, v))
+    ref, mag = _reference(q, k, v, left, right, sinks, False, q_start, skv)
+    _check(o, ref, mag)
+    token = O.window_attention(q, k, v, left, right, sinks=sinks, q_start=q_start, s_kv=skv, layout="token")
+    assert torch.equal(token.view(H, 1, D), o)
+
+
 @pytest.mark.parametrize("splits", [1, 2, 3, 7, 64])
 def test_any_number_of_splits(cuda_dev, splits):
     import h3attn as O
