@@ -13,11 +13,13 @@
 // the stacked B by TMA. So the adapters cost (64 * chunks) / k of the projection's products and no pass
 // over y. It is launched as a programmatic dependent: its first tiles run while lower_kernel finishes.
 //
-// Few rows (row path, two launches): bound by reading W once. stream_kernel: W and the stacked A are the M = 128
-// operand, the rows of x (16 .. 64 of them) the N operand; all their k-blocks, tile after tile, are dealt out
+// Few rows (row path, three launches): bound by reading W once. The weights are the M = 128 operand and the rows (16 ..
+// 64 of them) the N operand. few_lower_kernel: T, a cluster of 8 CTAs per 128 rows of the stacked A in use, an eighth of
+// k each, summed through distributed shared memory. stream_kernel: all k-blocks of W and, behind those of each
+// 128-row tile, the chunks in use of the same rows of the stacked B against T (as above); they are dealt out
 // evenly to two CTAs per SM, and each CTA writes fp32 sums of the piece of a tile that it had. finish_kernel adds a
-// column's pieces in a fixed order, then s_a B_a T with T in fp32, rounds and stores. Adapter tiles that no
-// row uses are neither read nor written.
+// column's pieces in a fixed order, rounds and stores. Each launch is a programmatic dependent of the one before:
+// W streams while T is made. (B T by scalar code in finish_kernel took 15-25 us at 37 rows x 21504 columns.)
 //
 // A row's value does not depend on the other rows of a call in either path (the paths differ in summation order).
 #include <algorithm>
@@ -257,63 +259,53 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAdapterThreads, 1)
   gemm_body<true>(tmap_x, tmap_w, tmap_b, p);
 }
 
-// ---------------------------------------------------------------- row path: W and A streamed once
-struct Stream {
-  int m, m_pad;           // rows, and rows rounded up to 16
-  int n_kb, kc_blocks;    // k-blocks of 64
-  int w_tiles, a_tiles;   // 128-row tiles of W, of the stacked A
-  int per_cta;            // k-blocks per CTA
+// ---------------------------------------------------------------- row path: T
+constexpr int kRing = 6;  // stages at most
+constexpr uint32_t kRingBytes = 6u * (kTileBytes + 16u * 128u);  // 108 KB: two CTAs per SM
+constexpr int kSplitK = 8;  // CTAs of a cluster, each an eighth of k
+
+struct Few {
+  int m, m_pad;         // rows, and rows rounded up to 16
+  int n_kb, kc_blocks;  // k-blocks of 64
   int stages;
-  float* part;            // [piece][m][columns]: column c of tile t at 128 t + c
-  long long columns;      // 128 * (w_tiles + a_tiles)
   int* status;
+  __nv_bfloat16* low;   // T [m][rank]
 };
-// The CTA that has k-block g of the tile list, and the first of a tile's CTAs: piece = cta - first_cta(tile).
-__device__ __forceinline__ int first_cta(const Stream& s, int tile) {
-  return int((long long)tile * s.n_kb / s.per_cta);
-}
-__device__ __forceinline__ int pieces_of(const Stream& s, int tile) {
-  return int(((long long)(tile + 1) * s.n_kb - 1) / s.per_cta) - first_cta(s, tile) + 1;
-}
 
-constexpr int kMaxStreamStages = 6;
-constexpr uint32_t kStreamRing = 6u * (kTileBytes + 16u * 128u);  // 108 KB: two CTAs per SM
-
-struct StreamSmem {
-  uint32_t used[kMaxChunks / 2 / 32];  // tiles of the stacked A that a row uses
-  uint64_t bars[2 * kMaxStreamStages + 5];
+struct FewLowerSmem {
+  uint64_t bars[2 * kRing + 2];
   uint32_t tmem;
-  int abort;
+  int abort, used;
 };
-constexpr uint32_t kStreamSmem = 1024 + kStreamRing + sizeof(StreamSmem);
+constexpr uint32_t kFewLowerSmem = 1024 + kRingBytes + sizeof(FewLowerSmem);
+static_assert(kRingBytes >= kFewRows * 128 * 4, "the sums reuse the ring");
 
 __global__ void __launch_bounds__(192, 2)
-    stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a,
-                  const __grid_constant__ CUtensorMap tmap_x, const Adapters ad, const Stream s) {
+    few_lower_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_x,
+                     const Adapters ad, const Few f) {
   pdl_launch_dependents();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
-  StreamSmem& sh = *reinterpret_cast<StreamSmem*>(smem + kStreamRing);
-  enum { kF = 0, kE = kMaxStreamStages, kAccF = 2 * kMaxStreamStages, kAccE = kAccF + 2, kD = kAccE + 2 };
+  FewLowerSmem& sh = *reinterpret_cast<FewLowerSmem*>(smem + kRingBytes);
+  enum { kF = 0, kE = kRing, kAcc = 2 * kRing, kD = kAcc + 1 };
   auto bar = [&](int i) { return smem_u32(&sh.bars[i]); };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t x_bytes = uint32_t(s.m_pad) * 128u, stage_bytes = kTileBytes + x_bytes;
-  // two accumulators of m_pad columns
-  const uint32_t cols = s.m_pad <= 16 ? 32u : (s.m_pad <= 32 ? 64u : 128u);
+  const int rank = int(cluster_ctarank());
+  const int tile = blockIdx.x / kSplitK;  // 128 rows of the stacked A
+  const uint32_t stage_bytes = kTileBytes + uint32_t(f.m_pad) * 128u;
+  const uint32_t cols = f.m_pad <= 32 ? 32u : 64u;
+  const int kb0 = f.n_kb * rank / kSplitK, kb1 = f.n_kb * (rank + 1) / kSplitK;
 
-  for (int i = threadIdx.x; i < kMaxChunks / 2 / 32; i += 192) sh.used[i] = 0;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kMaxStreamStages; ++i) {
+    for (int i = 0; i < kRing; ++i) {
       mbar_init(bar(kF + i), 1);
       mbar_init(bar(kE + i), 1);
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(bar(kAccF + b), 1);
-      mbar_init(bar(kAccE + b), 4);
-    }
+    mbar_init(bar(kAcc), 1);
     mbar_init(bar(kD), 1);
-    sh.abort = *reinterpret_cast<volatile int*>(s.status) != 0 ? 1 : 0;
+    sh.abort = *reinterpret_cast<volatile int*>(f.status) != 0 ? 1 : 0;
+    sh.used = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -321,125 +313,357 @@ __global__ void __launch_bounds__(192, 2)
     tmem_relinquish();
   }
   __syncthreads();
-  if (threadIdx.x < s.m) {
-    const int a = adapter_of(ad, s.m, threadIdx.x);
-    if (a >= 0) {
-      const int last = (a * ad.rank + ad.rank - 1) / 128;
-      for (int t = a * ad.rank / 128; t <= last; ++t) atomicOr(&sh.used[t / 32], 1u << (t & 31));
-    }
+  if (threadIdx.x < f.m) {  // does a row use an adapter with rows in this tile?
+    const int a = adapter_of(ad, f.m, threadIdx.x);
+    if (a >= 0 && a * ad.rank < 128 * (tile + 1) && (a + 1) * ad.rank > 128 * tile) sh.used = 1;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
-  const WaitCtx ctx{&sh.abort, s.status};
+  const WaitCtx ctx{&sh.abort, f.status};
+  const bool used = sh.used != 0;  // the same in every CTA of the cluster
+  const bool run = sh.abort == 0 && used && kb1 > kb0;
+
+  if (warp == 0 && run) {
+    const bool issuer = elect_one();
+    int it = 0;
+    for (int kb = kb0; kb < kb1; ++kb, ++it) {
+      const int st = it % f.stages;
+      if (it >= f.stages &&
+          !__all_sync(0xffffffffu, mbar_wait(bar(kE + st), uint32_t(it / f.stages - 1) & 1u, ctx, kStatusTimeoutKV)))
+        break;
+      if (issuer) {
+        const uint32_t dst = sbase + st * stage_bytes;
+        mbar_expect_tx(bar(kF + st), stage_bytes);
+        tma_load_3d(dst, &tmap_a, bar(kF + st), 64 * kb, 128 * tile, 0);
+        tma_load_3d(dst + kTileBytes, &tmap_x, bar(kF + st), 64 * (kb % f.kc_blocks), 0, kb / f.kc_blocks);
+      }
+      __syncwarp();
+    }
+    if (issuer)
+      for (int st = 0; st < f.stages; ++st) {
+        const int cnt = it / f.stages + (st < it % f.stages ? 1 : 0);
+        if (cnt > 0) drain_wait_cluster(bar(kF + st), uint32_t(cnt - 1) & 1u, f.status);
+      }
+    __syncwarp();
+  } else if (warp == 1 && run) {
+    const bool issuer = elect_one();
+    const uint32_t idesc = idesc_bf16_f32(128, f.m_pad, 0, 0);
+    int it = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb, ++it) {
+      const int st = it % f.stages;
+      if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar(kF + st), uint32_t(it / f.stages) & 1u, ctx, kStatusTimeoutKV))))
+        break;
+      tc_fence_after();
+      if (issuer) {
+        const uint32_t w = sbase + st * stage_bytes;
+        for (int ks = 0; ks < 4; ++ks)
+          mma_ss(tmem, smem_desc_sw128(w + 32u * ks, 16, 1024), smem_desc_sw128(w + kTileBytes + 32u * ks, 16, 1024),
+                 idesc, kb > kb0 || ks > 0 ? 1u : 0u);
+        mma_commit(bar(kE + st));
+      }
+      __syncwarp();
+    }
+    if (issuer) {
+      if (ok) mma_commit(bar(kAcc));
+      mma_commit(bar(kD));
+      drain_wait_cluster(bar(kD), 0, f.status);
+    }
+    __syncwarp();
+  }
+  // sums of this CTA's share of k to sums[row of x][row of the tile] (the ring is idle: every MMA has retired)
+  float* sums = reinterpret_cast<float*>(smem);
+  if (warp >= 2 && used) {
+    const int quad = warp & 3;
+    const bool ok = run && __all_sync(0xffffffffu, mbar_wait(bar(kAcc), 0, ctx, kStatusTimeoutS));
+    tc_fence_after();
+    for (int q = 0; q < f.m_pad / 16; ++q) {
+      uint32_t r[16];
+      if (ok) tmem_ld16_wait(tmem + (uint32_t(quad * 32) << 16) + 16u * q, r);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sums[(16 * q + e) * 128 + quad * 32 + lane] = ok ? __uint_as_float(r[e]) : 0.f;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (used && sh.abort == 0) {
+    // this CTA's sixteenth-row slices of the tile, over the cluster's sums in ascending order
+    constexpr int kMine = 128 / kSplitK;
+    for (int i = threadIdx.x; i < f.m * kMine; i += 192) {
+      const int row = i / kMine, at = kMine * rank + i % kMine;
+      const int g = 128 * tile + at, a = g / ad.rank;
+      if (adapter_of(ad, f.m, row) != a) continue;
+      float v = 0.f;
+#pragma unroll
+      for (int c = 0; c < kSplitK; ++c) v += ld_cluster_f32(mapa_shared(smem_u32(sums + row * 128 + at), c));
+      f.low[(long long)row * ad.rank + (g - a * ad.rank)] = __float2bfloat16_rn(v * ad.scale[a]);
+    }
+  }
+  cluster_sync_all();  // no CTA leaves while another reads its sums
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, cols);
+  }
+}
+
+// ---------------------------------------------------------------- row path: W and B streamed once
+struct Stream {
+  Few f;
+  int tiles;          // 128-row tiles of W
+  int* head;          // [2]: k-blocks per tile (those of W and the chunks in use), k-blocks per CTA
+  float* part;        // [piece][m][columns]
+  long long columns;  // 128 * tiles
+};
+// A tile's k-blocks [tile * per_tile, (tile + 1) * per_tile) of the whole list lie in CTAs first .. last; its pieces are
+// numbered from the first.
+__host__ __device__ inline int first_cta(int tile, int per_tile, int per_cta) {
+  return int((long long)tile * per_tile / per_cta);
+}
+__host__ __device__ inline int last_cta(int tile, int per_tile, int per_cta) {
+  return int(((long long)(tile + 1) * per_tile - 1) / per_cta);
+}
+
+constexpr int kStreamThreads = 256;  // TMA, MMA, 4 epilogue warps, 2 warps that write T
+constexpr int kFewChunks = kFewRows * (kMaxRank / 64);  // chunks in use at most
+
+struct StreamSmem {
+  uint32_t bits[kMaxChunks / 32];  // chunks in use
+  uint16_t list[kFewChunks];
+  int count;
+  uint64_t bars[4 * kRing + 5];
+  uint32_t tmem;
+  int abort;
+};
+constexpr uint32_t kStreamSmem = 1024 + kRingBytes + sizeof(StreamSmem);
+
+__global__ void __launch_bounds__(kStreamThreads, 2)
+    stream_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
+                  const __grid_constant__ CUtensorMap tmap_b, const Adapters ad, const Stream s) {
+  pdl_launch_dependents();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sbase = smem_u32(smem);
+  StreamSmem& sh = *reinterpret_cast<StreamSmem*>(smem + kRingBytes);
+  enum { kF = 0, kE = kRing, kLF = 2 * kRing, kLE = 3 * kRing, kAccF = 4 * kRing, kAccE = kAccF + 2, kD = kAccE + 2 };
+  auto bar = [&](int i) { return smem_u32(&sh.bars[i]); };
+  const Few& f = s.f;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t stage_bytes = kTileBytes + uint32_t(f.m_pad) * 128u;
+  // two accumulators of m_pad columns
+  const uint32_t cols = f.m_pad <= 16 ? 32u : (f.m_pad <= 32 ? 64u : 128u);
+
+  for (int i = threadIdx.x; i < kMaxChunks / 32; i += kStreamThreads) sh.bits[i] = 0;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(bar(kF + i), 1);
+      mbar_init(bar(kE + i), 1);
+      mbar_init(bar(kLE + i), 1);
+      mbar_init(bar(kLF + i), 2);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(bar(kAccF + b), 1);
+      mbar_init(bar(kAccE + b), 4);
+    }
+    mbar_init(bar(kD), 1);
+    sh.abort = *reinterpret_cast<volatile int*>(f.status) != 0 ? 1 : 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&sh.tmem), cols);
+    tmem_relinquish();
+  }
+  __syncthreads();
+  if (threadIdx.x < f.m) {
+    const int a = adapter_of(ad, f.m, threadIdx.x);
+    if (a >= 0) {
+      const int last = (a * ad.rank + ad.rank - 1) / 64;
+      for (int c = a * ad.rank / 64; c <= last; ++c) atomicOr(&sh.bits[c / 32], 1u << (c & 31));
+    }
+  }
+  __syncthreads();
+  if (warp == 2) {  // ascending list of the chunks in use
+    const uint32_t word = sh.bits[lane];
+    int at = __popc(word);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += up;
+    }
+    if (lane == 31) sh.count = at;
+    at -= __popc(word);
+    for (uint32_t w = word; w != 0; w &= w - 1, ++at) sh.list[at] = (uint16_t)(32 * lane + __ffs(w) - 1);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  const WaitCtx ctx{&sh.abort, f.status};
   const bool run = sh.abort == 0;
-  const long long total = (long long)(s.w_tiles + s.a_tiles) * s.n_kb;
-  const long long g_end = min(total, (long long)(blockIdx.x + 1) * s.per_cta);
-  auto skipped = [&](int tile) {
-    const int t = tile - s.w_tiles;
-    return t >= 0 && !((sh.used[t / 32] >> (t & 31)) & 1u);
+  const int per_tile = f.n_kb + sh.count;
+  const long long total = (long long)s.tiles * per_tile;
+  const int per_cta = int((total + gridDim.x - 1) / gridDim.x);
+  const long long g_begin = min(total, (long long)blockIdx.x * per_cta), g_end = min(total, g_begin + per_cta);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    s.head[0] = per_tile;
+    s.head[1] = per_cta;
+  }
+  // the CTA's pieces: k-blocks [kb0, kb1) of a tile
+  struct Piece {
+    int tile, kb0, kb1;
+  };
+  auto piece = [&](long long g) {
+    Piece q;
+    q.tile = int(g / per_tile);
+    q.kb0 = int(g - (long long)q.tile * per_tile);
+    q.kb1 = int(min((long long)per_tile, q.kb0 + (g_end - g)));
+    return q;
   };
 
   if (warp == 0 && run) {
     const bool issuer = elect_one();
     int it = 0;
     bool ok = true;
-    for (long long g = (long long)blockIdx.x * s.per_cta; ok && g < g_end;) {
-      const int tile = int(g / s.n_kb), kb0 = int(g - (long long)tile * s.n_kb);
-      const int kb1 = int(min((long long)s.n_kb, kb0 + (g_end - g)));
-      g += kb1 - kb0;
-      if (skipped(tile)) continue;
-      const bool is_w = tile < s.w_tiles;
-      const int row = 128 * (is_w ? tile : tile - s.w_tiles);
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int st = it % s.stages;
-        if (it >= s.stages && !(ok = __all_sync(0xffffffffu, mbar_wait(bar(kE + st), uint32_t(it / s.stages - 1) & 1u,
+    for (long long g = g_begin; ok && g < g_end;) {
+      const Piece q = piece(g);
+      g += q.kb1 - q.kb0;
+      for (int kb = q.kb0; kb < q.kb1; ++kb, ++it) {
+        const int st = it % f.stages;
+        if (it >= f.stages && !(ok = __all_sync(0xffffffffu, mbar_wait(bar(kE + st), uint32_t(it / f.stages - 1) & 1u,
                                                                        ctx, kStatusTimeoutKV))))
           break;
         if (issuer) {
           const uint32_t dst = sbase + st * stage_bytes;
-          mbar_expect_tx(bar(kF + st), stage_bytes);
-          tma_load_3d(dst, is_w ? &tmap_w : &tmap_a, bar(kF + st), 64 * kb, row, 0);
-          tma_load_3d(dst + kTileBytes, &tmap_x, bar(kF + st), 64 * (kb % s.kc_blocks), 0, kb / s.kc_blocks);
+          if (kb < f.n_kb) {
+            mbar_expect_tx(bar(kF + st), stage_bytes);
+            tma_load_3d(dst, &tmap_w, bar(kF + st), 64 * kb, 128 * q.tile, 0);
+            tma_load_3d(dst + kTileBytes, &tmap_x, bar(kF + st), 64 * (kb % f.kc_blocks), 0, kb / f.kc_blocks);
+          } else {
+            mbar_arrive(bar(kLE + st));
+            mbar_expect_tx(bar(kF + st), kTileBytes);
+            tma_load_3d(dst, &tmap_b, bar(kF + st), 64 * sh.list[kb - f.n_kb], 128 * q.tile, 0);
+          }
         }
         __syncwarp();
       }
     }
     if (issuer)
-      for (int st = 0; st < s.stages; ++st) {
-        const int cnt = it / s.stages + (st < it % s.stages ? 1 : 0);
-        if (cnt > 0) drain_wait_cluster(bar(kF + st), uint32_t(cnt - 1) & 1u, s.status);
+      for (int st = 0; st < f.stages; ++st) {
+        const int cnt = it / f.stages + (st < it % f.stages ? 1 : 0);
+        if (cnt > 0) drain_wait_cluster(bar(kF + st), uint32_t(cnt - 1) & 1u, f.status);
       }
     __syncwarp();
   } else if (warp == 1 && run) {
     const bool issuer = elect_one();
-    const uint32_t idesc = idesc_bf16_f32(128, s.m_pad, 0, 0);
+    const uint32_t idesc = idesc_bf16_f32(128, f.m_pad, 0, 0);
     int it = 0, i = 0;
+    uint32_t low_par = 0;  // bit st: parity of the stage's next use for T
     bool ok = true;
-    for (long long g = (long long)blockIdx.x * s.per_cta; ok && g < g_end;) {
-      const int tile = int(g / s.n_kb), kb0 = int(g - (long long)tile * s.n_kb);
-      const int kb1 = int(min((long long)s.n_kb, kb0 + (g_end - g)));
-      g += kb1 - kb0;
-      if (skipped(tile)) continue;
+    for (long long g = g_begin; ok && g < g_end; ++i) {
+      const Piece q = piece(g);
+      g += q.kb1 - q.kb0;
       const int b = i & 1;
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar(kAccE + b), (uint32_t(i >> 1) & 1u) ^ 1u, ctx, kStatusTimeoutO))))
         break;
       tc_fence_after();
-      for (int kb = kb0; kb < kb1; ++kb, ++it) {
-        const int st = it % s.stages;
+      for (int kb = q.kb0; kb < q.kb1; ++kb, ++it) {
+        const int st = it % f.stages;
         if (!(ok = __all_sync(0xffffffffu,
-                              mbar_wait(bar(kF + st), uint32_t(it / s.stages) & 1u, ctx, kStatusTimeoutKV))))
+                              mbar_wait(bar(kF + st), uint32_t(it / f.stages) & 1u, ctx, kStatusTimeoutKV))))
           break;
+        if (kb >= f.n_kb) {
+          if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar(kLF + st), (low_par >> st) & 1u, ctx, kStatusTimeoutKV))))
+            break;
+          low_par ^= 1u << st;
+        }
         tc_fence_after();
         if (issuer) {
           const uint32_t w = sbase + st * stage_bytes;
           for (int ks = 0; ks < 4; ++ks)
-            mma_ss(tmem + uint32_t(b * s.m_pad), smem_desc_sw128(w + 32u * ks, 16, 1024),
-                   smem_desc_sw128(w + kTileBytes + 32u * ks, 16, 1024), idesc, kb > kb0 || ks > 0 ? 1u : 0u);
+            mma_ss(tmem + uint32_t(b * f.m_pad), smem_desc_sw128(w + 32u * ks, 16, 1024),
+                   smem_desc_sw128(w + kTileBytes + 32u * ks, 16, 1024), idesc, kb > q.kb0 || ks > 0 ? 1u : 0u);
           mma_commit(bar(kE + st));
         }
         __syncwarp();
       }
       if (ok && issuer) mma_commit(bar(kAccF + b));
       __syncwarp();
-      ++i;
     }
     if (issuer) {
       mma_commit(bar(kD));
-      drain_wait_cluster(bar(kD), 0, s.status);
+      drain_wait_cluster(bar(kD), 0, f.status);
     }
     __syncwarp();
-  } else if (warp >= 2 && run) {
+  } else if (warp >= 2 && warp < 6 && run) {
     const int quad = warp & 3;
     const uint32_t lane_off = uint32_t(quad * 32) << 16;
     int i = 0;
     bool ok = true;
-    for (long long g = (long long)blockIdx.x * s.per_cta; ok && g < g_end;) {
-      const int tile = int(g / s.n_kb), kb0 = int(g - (long long)tile * s.n_kb);
-      const int kb1 = int(min((long long)s.n_kb, kb0 + (g_end - g)));
-      g += kb1 - kb0;
-      if (skipped(tile)) continue;
+    for (long long g = g_begin; ok && g < g_end; ++i) {
+      const Piece q = piece(g);
+      g += q.kb1 - q.kb0;
       const int b = i & 1;
       ok = __all_sync(0xffffffffu, mbar_wait(bar(kAccF + b), uint32_t(i >> 1) & 1u, ctx, kStatusTimeoutS));
       if (!ok) break;
       tc_fence_after();
       // lane = column of the tile: a warp stores 32 consecutive columns of a row
-      float* dst = s.part + (long long)(blockIdx.x - first_cta(s, tile)) * s.m * s.columns + 128ll * tile + quad * 32 + lane;
+      float* dst = s.part + (long long)((int)blockIdx.x - first_cta(q.tile, per_tile, per_cta)) * f.m * s.columns +
+                   128ll * q.tile + quad * 32 + lane;
 #pragma unroll 1
-      for (int q = 0; q < s.m_pad / 16; ++q) {
+      for (int c = 0; c < f.m_pad / 16; ++c) {
         uint32_t r[16];
-        tmem_ld16_wait(tmem + lane_off + uint32_t(b * s.m_pad + 16 * q), r);
+        tmem_ld16_wait(tmem + lane_off + uint32_t(b * f.m_pad + 16 * c), r);
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (16 * q + e < s.m) dst[(16 * q + e) * s.columns] = __uint_as_float(r[e]);
+          if (16 * c + e < f.m) dst[(16 * c + e) * s.columns] = __uint_as_float(r[e]);
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(kAccE + b));
-      ++i;
+    }
+  } else if (warp >= 6 && run && sh.count > 0) {
+    // T of a chunk: one thread per row of x, zeros outside the row's own adapter; K-major, 128-byte swizzle
+    const int row = (warp - 6) * 32 + lane;
+    const int a = adapter_of(ad, f.m, row);
+    const int col0 = a >= 0 ? a * ad.rank : -1;
+    const int pieces = min(ad.rank, 64) / 8;
+    const __nv_bfloat16* src = f.low + (long long)row * ad.rank;
+    uint32_t free_par = 0;
+    int it = 0;
+    bool ok = true;
+    pdl_wait();  // T comes from the kernel before
+    for (long long g = g_begin; ok && g < g_end;) {
+      const Piece q = piece(g);
+      g += q.kb1 - q.kb0;
+      it += max(0, min(q.kb1, f.n_kb) - q.kb0);
+      for (int kb = max(q.kb0, f.n_kb); kb < q.kb1; ++kb, ++it) {
+        const int st = it % f.stages;
+        const int first = 64 * sh.list[kb - f.n_kb];  // the chunk's first stacked column
+        const bool mine = col0 >= 0 && col0 < first + 64 && col0 + ad.rank > first;
+        const int at = max(col0 - first, 0) / 8;
+        const uint4* from = reinterpret_cast<const uint4*>(src + max(first - col0, 0));
+        uint4 v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[e] = make_uint4(0, 0, 0, 0);
+          if (mine && e >= at && e < at + pieces) v[e] = from[e - at];
+        }
+        if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar(kLE + st), (free_par >> st) & 1u, ctx, kStatusTimeoutKV)))) break;
+        free_par ^= 1u << st;
+        if (row < f.m_pad) {
+          const uint32_t dst = sbase + st * stage_bytes + kTileBytes + 128u * uint32_t(row);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) st_shared_u4(dst + (uint32_t(e ^ (row & 7)) << 4), v[e]);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(kLF + st));
+      }
     }
   }
+  pdl_wait();  // this grid has not finished before the one that it overlaps with
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -448,120 +672,53 @@ __global__ void __launch_bounds__(192, 2)
   }
 }
 
-// One row and 256 columns a CTA, two neighbouring columns a thread: the pieces of W x in ascending order, plus B_a T.
-// The first kAhead * 8 columns of B are loaded before the wait for stream_kernel (they do not depend on it).
-constexpr int kAhead = 4;
-
-struct Finish {
-  const __nv_bfloat16* b;  // stacked B
-  long long b_row;
-  __nv_bfloat16* c;
-  long long ldc;
-  int n_out, swiglu;
-};
-
-// Columns n and n + 1 of a row.
-struct FinishPair {
-  uint4 b0[kAhead], b1[kAhead];
-  const __nv_bfloat16* from;
-
-  __device__ __forceinline__ void load(const Finish& f, int col0, int rank, int n) {
-    from = f.b + n * f.b_row + col0;
-#pragma unroll
-    for (int q = 0; q < kAhead; ++q)
-      if (col0 >= 0 && 8 * q < rank) {
-        b0[q] = __ldg(reinterpret_cast<const uint4*>(from + 8 * q));
-        b1[q] = __ldg(reinterpret_cast<const uint4*>(from + f.b_row + 8 * q));
-      }
-  }
-  __device__ __forceinline__ float2 pieces(const Stream& s, int row, int n) const {
-    const int count = pieces_of(s, n / 128);
-    const float* at = s.part + row * s.columns + n;
-    float2 y = make_float2(0.f, 0.f);
+// Four neighbouring columns of a row a thread: the pieces in ascending order, rounded once.
+__device__ __forceinline__ float4 sum_pieces(const Stream& s, int per_tile, int per_cta, int row, int n) {
+  const int tile = n / 128;
+  const int count = last_cta(tile, per_tile, per_cta) - first_cta(tile, per_tile, per_cta) + 1;
+  const float* at = s.part + row * s.columns + n;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int q = 0; q < count; ++q) {
-      const float2 v = *reinterpret_cast<const float2*>(at + (long long)q * s.m * s.columns);
-      y.x += v.x;
-      y.y += v.y;
-    }
-    return y;
+  for (int q = 0; q < count; ++q) {
+    const float4 v = *reinterpret_cast<const float4*>(at + (long long)q * s.f.m * s.columns);
+    y.x += v.x;
+    y.y += v.y;
+    y.z += v.z;
+    y.w += v.w;
   }
-  static __device__ __forceinline__ void dot8(const uint4& u0, const uint4& u1, const float* t, float2& d) {
-    float w0[8], w1[8];
-    bf16x8_to_f32(u0, w0);
-    bf16x8_to_f32(u1, w1);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      d.x += w0[e] * t[e];
-      d.y += w1[e] * t[e];
-    }
-  }
-  __device__ __forceinline__ float2 low(const Finish& f, const float* t, int rank) const {
-    float2 d = make_float2(0.f, 0.f);
-#pragma unroll
-    for (int q = 0; q < kAhead; ++q)
-      if (8 * q < rank) dot8(b0[q], b1[q], t + 8 * q, d);
-    for (int j = 8 * kAhead; j < rank; j += 8)
-      dot8(__ldg(reinterpret_cast<const uint4*>(from + j)), __ldg(reinterpret_cast<const uint4*>(from + f.b_row + j)),
-           t + j, d);
-    return d;
-  }
-};
+  return y;
+}
 
-__global__ void __launch_bounds__(128) finish_kernel(const Adapters ad, const Stream s, const Finish f) {
-  __shared__ float t[kMaxRank];
-  const int row = blockIdx.y;
-  const int a = adapter_of(ad, s.m, row);
-  const int col0 = a < 0 ? -1 : a * ad.rank;
-  const int n = blockIdx.x * 256 + 2 * threadIdx.x;
-  const bool mine = n < f.n_out;
-  FinishPair y, u;
-  if (mine) y.load(f, col0, ad.rank, n);
-  if (mine && f.swiglu) u.load(f, col0, ad.rank, f.n_out + n);
+constexpr int kFinishThreads = 256;
+
+__global__ void __launch_bounds__(kFinishThreads)
+    finish_kernel(const Stream s, __nv_bfloat16* c, long long ldc, int n_out, int swiglu) {
   pdl_wait();
-  if (*reinterpret_cast<volatile int*>(s.status) != 0) return;
-  if (a >= 0) {
-    for (int j = threadIdx.x; j < ad.rank; j += 128) {
-      const int col = 128 * s.w_tiles + col0 + j;
-      const int count = pieces_of(s, col / 128);
-      float v = 0.f;
-#pragma unroll 4
-      for (int q = 0; q < count; ++q) v += s.part[((long long)q * s.m + row) * s.columns + col];
-      t[j] = v * ad.scale[a];
-    }
-  }
-  float2 gy = make_float2(0.f, 0.f), gu = gy;
-  if (mine) gy = y.pieces(s, row, n);
-  if (mine && f.swiglu) gu = u.pieces(s, row, f.n_out + n);
-  __syncthreads();
-  if (!mine) return;
-  if (a >= 0) {
-    const float2 d = y.low(f, t, ad.rank);
-    gy.x += d.x;
-    gy.y += d.y;
-  }
-  if (f.swiglu) {
-    if (a >= 0) {
-      const float2 d = u.low(f, t, ad.rank);
-      gu.x += d.x;
-      gu.y += d.y;
-    }
+  if (*reinterpret_cast<volatile int*>(s.f.status) != 0) return;
+  const int per_tile = s.head[0], per_cta = s.head[1];
+  const int row = blockIdx.y, n = 4 * (blockIdx.x * kFinishThreads + threadIdx.x);
+  if (n >= n_out) return;
+  float4 y = sum_pieces(s, per_tile, per_cta, row, n);
+  if (swiglu) {
     // out = bf16(bf16(silu(g)) * u), g and u the bf16-rounded gate / up projections
-    const float g0 = bf16_round(gy.x), g1 = bf16_round(gy.y);
-    gy.x = bf16_round(g0 / (1.0f + __expf(-g0))) * bf16_round(gu.x);
-    gy.y = bf16_round(g1 / (1.0f + __expf(-g1))) * bf16_round(gu.y);
+    const float4 u = sum_pieces(s, per_tile, per_cta, row, n_out + n);
+    auto gate = [](float g, float up) {
+      g = bf16_round(g);
+      return bf16_round(g / (1.0f + __expf(-g))) * bf16_round(up);
+    };
+    y = make_float4(gate(y.x, u.x), gate(y.y, u.y), gate(y.z, u.z), gate(y.w, u.w));
   }
-  *reinterpret_cast<uint32_t*>(f.c + (long long)row * f.ldc + n) = pack_bf16x2(gy.x, gy.y);
+  *reinterpret_cast<uint2*>(c + (long long)row * ldc + n) = make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
 }
 
 // ---------------------------------------------------------------- host
 struct Layout {
   bool few;
-  int64_t low_bytes, list_bytes, part_bytes;  // tile path: T, chunk lists; row path: pieces
+  int64_t low_bytes, list_bytes, part_bytes;  // T; chunk lists (tile path) or the two counts (row path); pieces
   int chunk_stride;
   Stream s;
-  int ctas;
-  int64_t bytes() const { return few ? part_bytes : low_bytes + list_bytes; }
+  int ctas, a_tiles;
+  int64_t bytes() const { return low_bytes + list_bytes + part_bytes; }
 };
 
 static int check_adapters(int64_t rank, int64_t n_adapters) {
@@ -574,27 +731,27 @@ static int make_layout(int64_t m, int64_t n_kb, int64_t kc_blocks, int64_t w_row
   l = {};
   const int64_t stacked = rank * n_adapters;
   l.few = m <= kFewRows;
+  l.low_bytes = (m * rank * 2 + 255) / 256 * 256;
   if (!l.few) {
     l.chunk_stride = 1 + (int)((stacked + 63) / 64);
-    l.low_bytes = (m * rank * 2 + 255) / 256 * 256;
     l.list_bytes = (m + 255) / 256 * l.chunk_stride * (int64_t)sizeof(int);
     return H3_OK;
   }
   int sms = 0, rc;
   if ((rc = sm_count(sms)) != H3_OK) return rc;
   Stream& s = l.s;
-  s.m = (int)m;
-  s.m_pad = (int)((m + 15) / 16 * 16);
-  s.n_kb = (int)n_kb;
-  s.kc_blocks = (int)kc_blocks;
-  s.w_tiles = (int)((w_rows + 127) / 128);
-  s.a_tiles = (int)((stacked + 127) / 128);
-  const int64_t total = (int64_t)(s.w_tiles + s.a_tiles) * n_kb;
-  s.per_cta = (int)((total + 2 * sms - 1) / (2 * sms));
-  l.ctas = (int)((total + s.per_cta - 1) / s.per_cta);
-  s.stages = std::min<int>(kMaxStreamStages, kStreamRing / (kTileBytes + s.m_pad * 128));
-  s.columns = 128ll * (s.w_tiles + s.a_tiles);
-  const int64_t most = (n_kb + s.per_cta - 2) / s.per_cta + 1;  // pieces of one tile
+  s.f.m = (int)m;
+  s.f.m_pad = (int)((m + 15) / 16 * 16);
+  s.f.n_kb = (int)n_kb;
+  s.f.kc_blocks = (int)kc_blocks;
+  s.f.stages = std::min<int>(kRing, kRingBytes / (kTileBytes + s.f.m_pad * 128));
+  s.tiles = (int)((w_rows + 127) / 128);
+  s.columns = 128ll * s.tiles;
+  l.a_tiles = (int)((stacked + 127) / 128);
+  // two CTAs per SM, four k-blocks each at least (a CTA's piece costs its write and its read)
+  l.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(2 * sms, s.tiles * n_kb / 4));
+  l.list_bytes = 256;
+  const int64_t most = (l.ctas + s.tiles - 1) / s.tiles + 2;  // pieces of a tile, whatever the chunks in use add
   l.part_bytes = most * m * s.columns * (int64_t)sizeof(float);
   return H3_OK;
 }
@@ -653,24 +810,42 @@ extern "C" int h3_gemm_adapters(const void* a, int64_t m, int64_t a_chunks, int6
   const Adapters ad = {row_adapter, scale, (int)n_adapters, (int)rank, (int)((stacked + 63) / 64)};
   CUtensorMap tx, tw, ta, tb;
   if ((rc = map_w(&tw, call)) != H3_OK) return rc;
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  __nv_bfloat16* low = reinterpret_cast<__nv_bfloat16*>(ws);
+  if ((rc = make_map(&tb, lora_b, stacked, w_rows, 1, lora_b_row_stride, w_rows * lora_b_row_stride)) != H3_OK) return rc;
   if (l.few) {
-    if ((rc = map_a(&tx, call, (unsigned)l.s.m_pad)) != H3_OK) return rc;
+    Stream& s = l.s;
+    s.f.status = status;
+    s.f.low = low;
+    s.head = reinterpret_cast<int*>(ws + l.low_bytes);
+    s.part = reinterpret_cast<float*>(ws + l.low_bytes + l.list_bytes);
+    if ((rc = map_a(&tx, call, (unsigned)s.f.m_pad)) != H3_OK) return rc;
     if ((rc = make_map(&ta, lora_a, k, stacked, 1, lora_a_row_stride, stacked * lora_a_row_stride)) != H3_OK) return rc;
-    l.s.part = reinterpret_cast<float*>(workspace);
-    l.s.status = status;
+    if ((rc = allow_smem(few_lower_kernel, kFewLowerSmem)) != H3_OK) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(l.a_tiles * kSplitK));
+    cfg.blockDim = dim3(192);
+    cfg.dynamicSmemBytes = kFewLowerSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = kSplitK;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, few_lower_kernel, ta, tx, ad, s.f) != cudaSuccess) return H3_ERR_LAUNCH;
     if ((rc = allow_smem(stream_kernel, kStreamSmem)) != H3_OK) return rc;
-    stream_kernel<<<(unsigned)l.ctas, 192, kStreamSmem, st>>>(tw, ta, tx, ad, l.s);
-    if (cudaGetLastError() != cudaSuccess) return H3_ERR_LAUNCH;
-    const Finish f = {reinterpret_cast<const __nv_bfloat16*>(lora_b), lora_b_row_stride,
-                      reinterpret_cast<__nv_bfloat16*>(c), c_row_stride, (int)n_out, epilogue};
-    const dim3 grid((unsigned)((n_out + 255) / 256), (unsigned)m);
-    return launch_dependent(finish_kernel, grid, 128, 0, st, ad, l.s, f);
+    if ((rc = launch_dependent(stream_kernel, dim3((unsigned)l.ctas), kStreamThreads, kStreamSmem, st, tw, tx, tb, ad,
+                               s)) != H3_OK)
+      return rc;
+    const dim3 grid((unsigned)((n_out / 4 + kFinishThreads - 1) / kFinishThreads), (unsigned)m);
+    return launch_dependent(finish_kernel, grid, kFinishThreads, 0, st, s, reinterpret_cast<__nv_bfloat16*>(c),
+                            (long long)c_row_stride, (int)n_out, (int)epilogue);
   }
   if ((rc = map_a(&tx, call)) != H3_OK) return rc;
   if ((rc = make_map(&ta, lora_a, k, stacked, 1, lora_a_row_stride, stacked * lora_a_row_stride, 64)) != H3_OK) return rc;
-  if ((rc = make_map(&tb, lora_b, stacked, w_rows, 1, lora_b_row_stride, w_rows * lora_b_row_stride)) != H3_OK) return rc;
-  __nv_bfloat16* low = reinterpret_cast<__nv_bfloat16*>(workspace);
-  int* chunks = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(workspace) + l.low_bytes);
+  int* chunks = reinterpret_cast<int*>(ws + l.low_bytes);
   if ((rc = allow_smem(lower_kernel, kLowerSmem)) != H3_OK) return rc;
   lower_kernel<<<(unsigned)((m + 127) / 128), 192, kLowerSmem, st>>>(tx, ta, ad, low, chunks, l.chunk_stride, (int)m,
                                                                      p.n_kb, p.kc_blocks, status);

@@ -638,6 +638,8 @@ def stack_adapters(pairs, scales, device=None):
     for A, B in pairs:
         if A.dim() != 2 or B.dim() != 2 or A.shape[1] != k or B.shape[0] != n or A.shape[0] != B.shape[1]:
             raise H3Error("adapters must be A [r, k], B [n, r] with one k and one n")
+        if not bool(torch.isfinite(B.to(torch.bfloat16)).all()):
+            raise H3Error("an adapter's B is not finite: it would reach the rows of other adapters")
     most = max(A.shape[0] for A, _ in pairs)
     rank = next((r for r in _RANKS if r >= most), None)
     if rank is None:
@@ -668,8 +670,8 @@ def linear_lora(a: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
       a, weight, out: as linear(); lora_a: [adapters * rank, k], lora_b: [weight rows, adapters * rank] bf16, adapter g at
       [g * rank, (g + 1) * rank) of both (stack_adapters lays them out); rank 8, 16, 32 or a multiple of 64 up to 256;
       scale: fp32 [adapters]; rows: int32 [m] (segment_rows makes it from token segments).
-    A row's bits do not depend on the other rows among calls of up to 64 rows, and among longer ones. In calls of more
-    than 64 rows B must be finite: rows of a 256-row block meet each other's adapters with zero weights."""
+    A row's bits do not depend on the other rows among calls of up to 64 rows, and among longer ones. B must be finite
+    where it is used: rows meet the adapters that share their group of 64 stacked columns with zero weights."""
     m, chunks, chunk_cols, chunk_stride, row_stride, n, ep, out = _linear_args(a, weight, out, epilogue)
     _cuda(lora_a, "lora_a")
     _cuda(lora_b, "lora_b")

@@ -152,28 +152,30 @@ def test_stack_adapters():
     assert a.shape == (64, 40) and b.shape == (16, 64) and s.tolist() == [1.0, 0.5]
     assert torch.equal(a[:3], A[0].bfloat16()) and not a[3:32].any() and torch.equal(a[32:52], A[1].bfloat16())
     assert torch.equal(b[:, 32:52], B[1].bfloat16()) and not b[:, 52:].any()
-    for bad in (([], []), ([(A[0], B[0])], [1, 2]), ([(A[0], B[1])], [1]), ([(torch.zeros(300, 8), torch.zeros(8, 300))], [1])):
+    for bad in (([], []), ([(A[0], B[0])], [1, 2]), ([(A[0], B[1])], [1]), ([(torch.zeros(300, 8), torch.zeros(8, 300))], [1]),
+                ([(A[0], B[0] * float("nan"))], [1])):
         with pytest.raises(O.H3Error):
             O.stack_adapters(*bad)
 
 
-@pytest.mark.parametrize("tiles,n_kb,ctas", [(1, 1, 296), (171, 84, 296), (43, 112, 296), (253, 4, 296), (9, 3, 8),
-                                             (2, 1000, 7)])
-def test_streamed_blocks_are_dealt_once(tiles, n_kb, ctas):
+@pytest.mark.parametrize("tiles,n_kb,chunks,sms", [(1, 1, 0, 148), (168, 84, 6, 148), (42, 112, 1, 148),
+                                                   (252, 4, 256, 148), (9, 3, 2, 4), (2, 1000, 0, 3), (7, 30, 40, 148)])
+def test_streamed_blocks_are_dealt_once(tiles, n_kb, chunks, sms):
     """The row path's split of (tile, k-block) over CTAs, restated: every block in one CTA, a tile's pieces numbered
-    from 0 without gaps, and never more of them than the workspace holds."""
-    total = tiles * n_kb
+    from 0 without gaps, and never more of them than the workspace holds, whatever the chunks in use add."""
+    ctas = max(1, min(2 * sms, tiles * n_kb // 4))
+    most = -(-ctas // tiles) + 2
+    per_tile = n_kb + chunks
+    total = tiles * per_tile
     per = -(-total // ctas)
-    most = (n_kb + per - 2) // per + 1
     seen = set()
-    for cta in range(-(-total // per)):
-        g = cta * per
-        while g < min(total, (cta + 1) * per):
-            tile, kb0 = divmod(g, n_kb)
-            kb1 = min(n_kb, kb0 + min(total, (cta + 1) * per) - g)
-            piece = cta - tile * n_kb // per
-            count = ((tile + 1) * n_kb - 1) // per - tile * n_kb // per + 1
-            assert 0 <= piece < count <= most
+    for cta in range(ctas):
+        g, end = min(total, cta * per), min(total, cta * per + per)
+        while g < end:
+            tile, kb0 = divmod(g, per_tile)
+            kb1 = min(per_tile, kb0 + end - g)
+            first, last = tile * per_tile // per, ((tile + 1) * per_tile - 1) // per
+            assert 0 <= cta - first <= last - first < most
             for kb in range(kb0, kb1):
                 assert (tile, kb) not in seen
                 seen.add((tile, kb))
