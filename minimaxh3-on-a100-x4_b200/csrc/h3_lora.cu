@@ -19,7 +19,7 @@
 // 128-row tile, the chunks in use of the same rows of the stacked B against T (as above); they are dealt out
 // evenly to two CTAs per SM, and each CTA writes fp32 sums of the piece of a tile that it had. finish_kernel adds a
 // column's pieces in a fixed order, rounds and stores. Each launch is a programmatic dependent of the one before:
-// W streams while T is made. (B T by scalar code in finish_kernel took 15-25 us at 37 rows x 21504 columns.)
+// W streams while T is made, and a CTA leaves its piece with B for last. (B T by scalar code in finish_kernel took 15-25 us at 37 rows x 21504 columns.)
 //
 // A row's value does not depend on the other rows of a call in either path (the paths differ in summation order).
 #include <algorithm>
@@ -260,8 +260,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kAdapterThreads, 1)
 }
 
 // ---------------------------------------------------------------- row path: T
-constexpr int kRing = 6;  // stages at most
-constexpr uint32_t kRingBytes = 6u * (kTileBytes + 16u * 128u);  // 108 KB: two CTAs per SM
+constexpr int kRing = 4;  // stages at most
+// 72 KB, three to four stages: two CTAs of stream_kernel and one of few_lower_kernel fit an SM, so that no CTA of the
+// first waits for the second to leave (with 108 KB rings that cost 4-5 us of 24-51).
+constexpr uint32_t kRingBytes = 72u * 1024u;
 constexpr int kSplitK = 8;  // CTAs of a cluster, each an eighth of k
 
 struct Few {
@@ -510,15 +512,18 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     s.head[0] = per_tile;
     s.head[1] = per_cta;
   }
-  // the CTA's pieces: k-blocks [kb0, kb1) of a tile
+  // the CTA's pieces, k-blocks [kb0, kb1) of a tile, from the last to the first: the start of a tile, whole ones, the
+  // end of one with its chunks of B
   struct Piece {
     int tile, kb0, kb1;
   };
-  auto piece = [&](long long g) {
+  auto piece = [&](long long& g) {  // the piece that ends at g; g becomes its begin
     Piece q;
-    q.tile = int(g / per_tile);
-    q.kb0 = int(g - (long long)q.tile * per_tile);
-    q.kb1 = int(min((long long)per_tile, q.kb0 + (g_end - g)));
+    q.tile = int((g - 1) / per_tile);
+    const long long base = (long long)q.tile * per_tile;
+    q.kb1 = int(g - base);
+    q.kb0 = int(max(0ll, g_begin - base));
+    g = base + q.kb0;
     return q;
   };
 
@@ -526,9 +531,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     const bool issuer = elect_one();
     int it = 0;
     bool ok = true;
-    for (long long g = g_begin; ok && g < g_end;) {
+    for (long long g = g_end; ok && g > g_begin;) {
       const Piece q = piece(g);
-      g += q.kb1 - q.kb0;
       for (int kb = q.kb0; kb < q.kb1; ++kb, ++it) {
         const int st = it % f.stages;
         if (it >= f.stages && !(ok = __all_sync(0xffffffffu, mbar_wait(bar(kE + st), uint32_t(it / f.stages - 1) & 1u,
@@ -561,9 +565,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     int it = 0, i = 0;
     uint32_t low_par = 0;  // bit st: parity of the stage's next use for T
     bool ok = true;
-    for (long long g = g_begin; ok && g < g_end; ++i) {
+    for (long long g = g_end; ok && g > g_begin; ++i) {
       const Piece q = piece(g);
-      g += q.kb1 - q.kb0;
       const int b = i & 1;
       if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar(kAccE + b), (uint32_t(i >> 1) & 1u) ^ 1u, ctx, kStatusTimeoutO))))
         break;
@@ -601,9 +604,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     const uint32_t lane_off = uint32_t(quad * 32) << 16;
     int i = 0;
     bool ok = true;
-    for (long long g = g_begin; ok && g < g_end; ++i) {
+    for (long long g = g_end; ok && g > g_begin; ++i) {
       const Piece q = piece(g);
-      g += q.kb1 - q.kb0;
       const int b = i & 1;
       ok = __all_sync(0xffffffffu, mbar_wait(bar(kAccF + b), uint32_t(i >> 1) & 1u, ctx, kStatusTimeoutS));
       if (!ok) break;
@@ -634,9 +636,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     int it = 0;
     bool ok = true;
     pdl_wait();  // T comes from the kernel before
-    for (long long g = g_begin; ok && g < g_end;) {
+    for (long long g = g_end; ok && g > g_begin;) {
       const Piece q = piece(g);
-      g += q.kb1 - q.kb0;
       it += max(0, min(q.kb1, f.n_kb) - q.kb0);
       for (int kb = max(q.kb0, f.n_kb); kb < q.kb1; ++kb, ++it) {
         const int st = it % f.stages;
