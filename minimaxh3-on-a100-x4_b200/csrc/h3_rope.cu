@@ -16,7 +16,7 @@
 // (or a share of its rows, when there are fewer tokens than warps): each lane evaluates two of the
 // 64 sine/cosine pairs, the warp exchanges them through shared memory, and its four 8-lane groups
 // take one head row each (16 elements a lane, 16-byte accesses, both halves of a pair in one lane),
-// kRows rows a group in flight.
+// two (pack) or four rows a group in flight. rope_axes: 89 us at 40868 tokens x 28 heads = 6.6 TB/s, the copy rate.
 #include "h3_rows.cuh"
 #include "h3attn.h"
 
@@ -55,10 +55,8 @@ __device__ __forceinline__ LanePairs lane_pairs(const Axes& ax, int lane) {
   return lp;
 }
 
-// cos / sin of the token's 64 angles into the warp's 64 float2 of shared memory, then this lane's
-// eight pairs (8g .. 8g+7) into registers.
-__device__ __forceinline__ void token_angles(const Axes& ax, const LanePairs& lp, long long tok, int lane, int g,
-                                             float2* sh, float (&c)[8], float (&s)[8]) {
+// cos / sin of the token's 64 angles into the warp's 64 float2 of shared memory.
+__device__ __forceinline__ void token_angles(const Axes& ax, const LanePairs& lp, long long tok, int lane, float2* sh) {
   __syncwarp();  // the previous token's pairs have been read
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -74,6 +72,10 @@ __device__ __forceinline__ void token_angles(const Axes& ax, const LanePairs& lp
     sh[lane + 32 * i] = cs;
   }
   __syncwarp();
+}
+
+// This lane's eight pairs (8g .. 8g+7) of them.
+__device__ __forceinline__ void lane_angles(const float2* sh, int g, float (&c)[8], float (&s)[8]) {
   const float4* src = reinterpret_cast<const float4*>(sh + 8 * g);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -107,7 +109,8 @@ __global__ void __launch_bounds__(32 * kWarps, 3)
     const int h0 = int(it - tok * parts) * part_heads;
     const int h1 = min(h0 + part_heads, n_heads);
     float c[8], s[8];
-    token_angles(ax, lp, tok, lane, g, sh_cs[warp], c, s);
+    token_angles(ax, lp, tok, lane, sh_cs[warp]);
+    lane_angles(sh_cs[warp], g, c, s);
     for (int base = h0; base < h1; base += kStep) {
       uint4 u[kRows][2];
 #pragma unroll
@@ -136,19 +139,52 @@ __global__ void __launch_bounds__(32 * kWarps, 3)
   }
 }
 
+// One head row of an 8-lane group in place: y = x / sqrt(mean(x^2) + eps) * w, then the rotation. Lane g holds elements
+// [8g, 8g + 8) and [64 + 8g, ...); weights and angles stay packed (bf16 words, shared memory), so that the row itself is
+// all that a thread keeps in fp32.
+__device__ __forceinline__ void norm_turn_row(uint4& u0, uint4& u1, const uint4& w0, const uint4& w1, const float4* cs,
+                                              float eps) {
+  float v[16];
+  bf16x8_to_f32(u0, v);
+  bf16x8_to_f32(u1, v + 8);
+  float q = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) q += v[e] * v[e];
+  q += __shfl_xor_sync(0xffffffffu, q, 4);
+  q += __shfl_xor_sync(0xffffffffu, q, 2);
+  q += __shfl_xor_sync(0xffffffffu, q, 1);
+  const float r = 1.0f / sqrtf(q * (1.0f / kHeadDim) + eps);
+  const uint32_t wa[4] = {w0.x, w0.y, w0.z, w0.w}, wb[4] = {w1.x, w1.y, w1.z, w1.w};
+  uint32_t oa[4], ob[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float4 t = cs[j];
+    const float a0 = v[2 * j] * r * __uint_as_float(wa[j] << 16);
+    const float a1 = v[2 * j + 1] * r * __uint_as_float(wa[j] & 0xFFFF0000u);
+    const float b0 = v[8 + 2 * j] * r * __uint_as_float(wb[j] << 16);
+    const float b1 = v[9 + 2 * j] * r * __uint_as_float(wb[j] & 0xFFFF0000u);
+    oa[j] = pack_bf16x2(t.x * a0 - t.y * b0, t.z * a1 - t.w * b1);
+    ob[j] = pack_bf16x2(t.y * a0 + t.x * b0, t.w * a1 + t.z * b1);
+  }
+  u0 = make_uint4(oa[0], oa[1], oa[2], oa[3]);
+  u1 = make_uint4(ob[0], ob[1], ob[2], ob[3]);
+}
+
 struct PackOut {
   __nv_bfloat16* base[3];  // q, k, v (one local send buffer)
   long long rank_stride, head_stride;
   const unsigned long long* rank_base;  // or one buffer per destination rank (peer memory)
   long long tensor_stride, row_offset;
   int heads_per_rank;
+  unsigned rank_magic;  // ceil(2^32 / heads_per_rank): h / heads_per_rank = h * magic >> 32 for h < 2^16 (one rank: 0)
 };
-__device__ __forceinline__ __nv_bfloat16* pack_row(const PackOut& o, int tensor, int h, long long tok) {
-  const int r = h / o.heads_per_rank, hl = h - r * o.heads_per_rank;
+template <int kTensor>
+__device__ __forceinline__ __nv_bfloat16* pack_row(const PackOut& o, int h, long long tok) {
+  const int r = int(__umulhi((unsigned)h, o.rank_magic)), hl = h - r * o.heads_per_rank;
   return o.rank_base != nullptr
-             ? reinterpret_cast<__nv_bfloat16*>(o.rank_base[r]) + tensor * o.tensor_stride +
+             ? reinterpret_cast<__nv_bfloat16*>(o.rank_base[r]) + kTensor * o.tensor_stride +
                    (long long)hl * o.head_stride + (o.row_offset + tok) * kHeadDim
-             : o.base[tensor] + (long long)r * o.rank_stride + (long long)hl * o.head_stride + tok * kHeadDim;
+             : o.base[kTensor] + (long long)r * o.rank_stride + (long long)hl * o.head_stride + tok * kHeadDim;
 }
 
 // in[0..2]: q, k, v rows; w[0..1]: the RMSNorm weights of q and k or nullptr.
@@ -159,9 +195,52 @@ struct PackIn {
   float eps;
 };
 
-__global__ void __launch_bounds__(32 * kWarps, 2)
-    pack_axes_kernel(const PackIn in, const Axes ax, const PackOut out, long long tokens, int n_heads, int parts,
-                     int part_heads) {
+// Two rows in flight a group and three CTAs (24 warps) an SM, 80 registers without spills: 588 us at 42000 tokens x 56
+// heads = 6.14 TB/s, 0.94 of the copy rate. Four rows at two CTAs: 639 us, two rows at four CTAs (spills): 585 us there
+// but 92 against 83 us at 5250 tokens, one row at five: 634 us. (Weights and angles in registers as fp32, four rows:
+// 720 us; parameter arrays indexed by a runtime tensor number, which go through local memory: 690 us.)
+constexpr int kPackRows = 2;                // head rows in flight per 8-lane group
+constexpr int kPackStep = 4 * kPackRows;
+constexpr int kPackCtas = 3;                // CTAs per SM
+
+// Heads [h0, h1) of one token and one of q, k, v (0, 1, 2; v is copied).
+template <int kTensor>
+__device__ __forceinline__ void pack_heads(const PackIn& in, const PackOut& out, const float4* cs, long long tok, int h0,
+                                           int h1, int g, int grp) {
+  uint4 w0 = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u), w1 = w0;  // bf16 ones
+  if constexpr (kTensor < 2) {
+    if (in.w[kTensor] != nullptr) {
+      w0 = __ldg(reinterpret_cast<const uint4*>(in.w[kTensor] + 8 * g));
+      w1 = __ldg(reinterpret_cast<const uint4*>(in.w[kTensor] + 64 + 8 * g));
+    }
+  }
+  const __nv_bfloat16* src0 = in.in[kTensor] + tok * in.row_stride + 8 * g;
+#pragma unroll 1
+  for (int base = h0; base < h1; base += kPackStep) {
+    uint4 u[kPackRows][2];
+#pragma unroll
+    for (int i = 0; i < kPackRows; ++i) {
+      const int h = min(base + 4 * i + grp, h1 - 1);  // every lane joins the shuffles below
+      const __nv_bfloat16* src = src0 + h * kHeadDim;
+      u[i][0] = __ldg(reinterpret_cast<const uint4*>(src));
+      u[i][1] = __ldg(reinterpret_cast<const uint4*>(src + 64));
+    }
+#pragma unroll
+    for (int i = 0; i < kPackRows; ++i) {
+      if constexpr (kTensor < 2) norm_turn_row(u[i][0], u[i][1], w0, w1, cs, in.eps);
+      const int h = base + 4 * i + grp;
+      if (h < h1) {
+        __nv_bfloat16* dst = pack_row<kTensor>(out, h, tok) + 8 * g;
+        *reinterpret_cast<uint4*>(dst) = u[i][0];
+        *reinterpret_cast<uint4*>(dst + 64) = u[i][1];
+      }
+    }
+  }
+}
+
+__global__ void __launch_bounds__(32 * kWarps, kPackCtas)
+    pack_axes_kernel(const __grid_constant__ PackIn in, const __grid_constant__ Axes ax,
+                     const __grid_constant__ PackOut out, long long tokens, int n_heads, int parts, int part_heads) {
   __shared__ float2 sh_cs[kWarps][64];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane & 7, grp = lane >> 3;
@@ -171,57 +250,11 @@ __global__ void __launch_bounds__(32 * kWarps, 2)
     const long long tok = it / parts;
     const int h0 = int(it - tok * parts) * part_heads;
     const int h1 = min(h0 + part_heads, n_heads);
-    float c[8], s[8];
-    token_angles(ax, lp, tok, lane, g, sh_cs[warp], c, s);
-#pragma unroll 1
-    for (int tensor = 0; tensor < 3; ++tensor) {
-      float w[16];
-      if (tensor < 2) {
-        if (in.w[tensor] != nullptr) {
-          bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(in.w[tensor] + 8 * g)), w);
-          bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(in.w[tensor] + 64 + 8 * g)), w + 8);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = 1.0f;
-        }
-      }
-      for (int base = h0; base < h1; base += kStep) {
-        uint4 u[kRows][2];
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-          const int h = min(base + 4 * i + grp, h1 - 1);  // every lane joins the shuffles below
-          const __nv_bfloat16* src = in.in[tensor] + tok * in.row_stride + (long long)h * kHeadDim + 8 * g;
-          u[i][0] = __ldg(reinterpret_cast<const uint4*>(src));
-          u[i][1] = __ldg(reinterpret_cast<const uint4*>(src + 64));
-        }
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-          if (tensor < 2) {
-            float v[16];
-            bf16x8_to_f32(u[i][0], v);
-            bf16x8_to_f32(u[i][1], v + 8);
-            float q = 0.f;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) q += v[e] * v[e];
-            q += __shfl_xor_sync(0xffffffffu, q, 4);
-            q += __shfl_xor_sync(0xffffffffu, q, 2);
-            q += __shfl_xor_sync(0xffffffffu, q, 1);
-            const float r = 1.0f / sqrtf(q * (1.0f / kHeadDim) + in.eps);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) v[e] = v[e] * r * w[e];
-            rotate(v, c, s);
-            u[i][0] = f32_to_bf16x8(v);
-            u[i][1] = f32_to_bf16x8(v + 8);
-          }
-          const int h = base + 4 * i + grp;
-          if (h < h1) {
-            __nv_bfloat16* dst = pack_row(out, tensor, h, tok) + 8 * g;
-            *reinterpret_cast<uint4*>(dst) = u[i][0];
-            *reinterpret_cast<uint4*>(dst + 64) = u[i][1];
-          }
-        }
-      }
-    }
+    token_angles(ax, lp, tok, lane, sh_cs[warp]);
+    const float4* cs = reinterpret_cast<const float4*>(sh_cs[warp] + 8 * g);  // (cos, sin) of pairs 8g + 2j, 8g + 2j + 1
+    pack_heads<0>(in, out, cs, tok, h0, h1, g, grp);
+    pack_heads<1>(in, out, cs, tok, h0, h1, g, grp);
+    pack_heads<2>(in, out, cs, tok, h0, h1, g, grp);
   }
   if (out.rank_base != nullptr) __threadfence_system();  // peer stores visible before the host-side barrier
 }
@@ -243,17 +276,19 @@ static int make_axes(const void* pos, int32_t pos_type, int64_t n_axes, const do
   return H3_OK;
 }
 
-// One warp a token; with fewer tokens than the GPU holds warps, a token's heads are split over several.
+// One warp a token; below 64 tokens an SM a token's heads are split over several warps, so that the SMs' resident warps
+// (24 an SM) come round two or three times and the last round is short: 5250 tokens x 56 heads, 90 us without, 80
+// with; 1500 tokens, 27 us, 43 with twice as many parts. Four heads a part at least (a warp's rows at a time).
 static int head_parts(int64_t tokens, int64_t n_heads, int& parts, int& part_heads) {
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return H3_ERR_CUDA;
-  const int64_t warps = (int64_t)sms * 2 * kWarps;
-  int64_t want = tokens >= warps ? 1 : (warps + tokens - 1) / tokens;
-  const int64_t most = (n_heads + 3) / 4;  // four rows a warp step at least
-  if (want > most) want = most;
-  part_heads = (int)(((n_heads + want - 1) / want + 3) / 4 * 4);
-  parts = (int)((n_heads + part_heads - 1) / part_heads);
+  const int64_t warps = (int64_t)sms * 64;
+  const int64_t want = tokens >= warps ? 1 : (warps + tokens - 1) / tokens;
+  int64_t heads = ((n_heads + want - 1) / want + 3) / 4 * 4;
+  if (heads > kPackStep) heads = (heads + kPackStep - 1) / kPackStep * kPackStep;  // whole steps
+  part_heads = (int)heads;
+  parts = (int)((n_heads + heads - 1) / heads);
   return H3_OK;
 }
 
@@ -276,6 +311,7 @@ static int pack_impl(const void* q, const void* k, const void* v, int64_t in_row
   in.w[1] = reinterpret_cast<const __nv_bfloat16*>(k_weight);
   in.eps = eps;
   o.heads_per_rank = (int)heads_per_rank;
+  o.rank_magic = heads_per_rank == n_heads ? 0u : (unsigned)(((1ull << 32) + heads_per_rank - 1) / heads_per_rank);
   int parts = 1, part_heads = 1, rc;
   if ((rc = head_parts(s_l, n_heads, parts, part_heads)) != H3_OK) return rc;
   pack_axes_kernel<<<grid_for(s_l * parts, kWarps, 1 << 20), 32 * kWarps, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
@@ -325,7 +361,7 @@ extern "C" int h3_qknorm_rope_pack_axes(const void* q, const void* k, const void
   if (out_rank_stride % 8) return H3_ERR_STRIDE;
   PackOut o = {{reinterpret_cast<__nv_bfloat16*>(q_out), reinterpret_cast<__nv_bfloat16*>(k_out),
                 reinterpret_cast<__nv_bfloat16*>(v_out)},
-               out_rank_stride, out_head_stride, nullptr, 0, 0, 1};
+               out_rank_stride, out_head_stride, nullptr, 0, 0, 1, 0};
   return pack_impl(q, k, v, in_row_stride, ax, q_weight, k_weight, eps, o, s_l, n_heads, heads_per_rank, stream);
 }
 
@@ -345,6 +381,6 @@ extern "C" int h3_qknorm_rope_pack_axes_peer(const void* q, const void* k, const
   if (row_offset < 0 || heads_per_rank < 1 || n_ranks < 1 || n_heads / heads_per_rank > n_ranks) return H3_ERR_SHAPE;
   if ((tensor_stride % 8) || tensor_stride < 0 || head_stride < 0) return H3_ERR_STRIDE;
   PackOut o = {{nullptr, nullptr, nullptr}, 0, head_stride, reinterpret_cast<const unsigned long long*>(rank_base),
-               tensor_stride, row_offset, 1};
+               tensor_stride, row_offset, 1, 0};
   return pack_impl(q, k, v, in_row_stride, ax, q_weight, k_weight, eps, o, s_l, n_heads, heads_per_rank, stream);
 }
