@@ -181,3 +181,30 @@ def test_streamed_blocks_are_dealt_once(tiles, n_kb, chunks, sms):
                 seen.add((tile, kb))
             g += kb1 - kb0
     assert len(seen) == total
+
+
+def test_launch_order_of_query_blocks():
+    """The window kernel's launch order, restated: every (block, head) once; the middle first, then the ends from the
+    middle outwards, where walks get shorter."""
+    import itertools
+
+    def block_of(w, blocks, first, mid, heads, turn):
+        if w < mid * heads:
+            return first + w % mid, w // mid
+        ends, u = blocks - mid, w - mid * heads
+        kvh, k = (u % heads, u // heads) if turn else (u // ends, u % ends)
+        before, behind = first, ends - first
+        both = 2 * min(before, behind)
+        i = k >> 1 if k < both else k - (both >> 1)
+        front = k % 2 == 0 if k < both else before > behind
+        return (before - 1 - i if front else first + mid + i), kvh
+
+    for blocks in range(1, 9):
+        for first in range(blocks + 1):
+            for mid in range(blocks - first + 1):
+                for heads, turn in itertools.product((1, 3), (False, True)):
+                    got = [block_of(w, blocks, first, mid, heads, turn) for w in range(blocks * heads)]
+                    assert sorted(got) == sorted(itertools.product(range(blocks), range(heads)))
+                    for h in range(heads):
+                        far = [max(first - b, b - first - mid + 1, 0) for b, kvh in got if kvh == h]
+                        assert far == sorted(far)
