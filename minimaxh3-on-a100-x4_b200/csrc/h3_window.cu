@@ -18,10 +18,18 @@
 // tile) have their V rows zeroed in shared memory before the product, so whatever a cache
 // holds there cannot reach a result through 0 * NaN.
 //
-// kTiles = 2: CTA = 256 packed rows, 12 warps, 5-stage K/V ring, one CTA per SM (the full kernel's
-// schedule). kTiles = 1: CTA = 128 packed rows, 8 warps, 2-stage ring, two CTAs per SM. Few rows split the tile
-// list over gridDim.z CTAs; each writes (O, m, l) in fp32 to the caller's workspace and join_kernel
-// combines them in a fixed order. A single token has a kernel of its own (token_kernel).
+// kTiles = 2: 256 packed rows a work item, 12 warps, 5-stage K/V ring, one CTA per SM (the full kernel's schedule). CTAs
+// are persistent: the ring runs on across items, the next item's Q loads once the last Q K^T of this one has retired, and
+// its first S is issued behind the last P V, so that only the write-back of O is left between two items (with a CTA
+// per item a start and an end cost 10 us of a 28 us item; 37 heads x 8192, window 511 + 512: 227 us, 206 so). kTiles = 1:
+// 128 packed rows, 8 warps, 2-stage ring, two CTAs per SM, a CTA per item. Few rows split the tile list over several
+// items; each writes (O, m, l) in fp32 to the caller's workspace and join_kernel combines them in a fixed order. A
+// single token has a kernel of its own (token_kernel).
+//
+// Bound: 42000 queries x 14 heads, window 2048 + 2048, 512 first tokens: 1.20 ms = 1122 TFLOP/s of visible pairs before
+// the power cap, 1.30-1.36 ms (1.0 PFLOP/s) under it; the exponentials and the chain S -> P -> O of a tile bound it, as in
+// the full kernel (1.85 us per 256 x 128 tile). A masked tile costs 0.09 us more. Short windows are bound by the walk's
+// start: 28 heads x 4096, window 511 + 512: 96 us. 5 tokens x 56 heads over 168000 keys of 8 heads: 116 us = 5.9 TB/s.
 #include <algorithm>
 #include <cmath>
 
@@ -39,6 +47,7 @@ struct Params {
   // blocks of queries in the order of launch: those in the middle of the sequence, head by head, then the ones at its
   // ends, whose walks are shorter, from the longest down
   int blocks, first_mid, n_mid, kv_heads, heads_turn;
+  int splits, n_items, rounds;  // work items: (block, part); rounds of the grid over them
   float scale_log2;
   __nv_bfloat16* o;
   long long o_rank_rows, o_rank_stride, o_head_stride, o_row_stride;
@@ -87,6 +96,49 @@ __device__ __forceinline__ void block_of(const Params& p, int w, int& block, int
   block = front ? before - 1 - i : p.first_mid + p.n_mid + i;
 }
 
+// One work item: a block of queries of one key head, and part z of its key tiles, [j_lo, j_lo + n_kv) of the walk.
+struct Item {
+  int kvh, i0, z;
+  int j_lo, n_kv;
+};
+// Work item of this CTA in round r, or -1. Rounds alternate in direction: items are in descending length, so that a CTA's
+// long and short ones even out.
+template <int kTiles>
+__device__ __forceinline__ int rounds_of(const Params& p) {
+  return kTiles == 1 ? 1 : p.rounds;  // one Q tile: a CTA per item
+}
+template <int kTiles>
+__device__ __forceinline__ int item_of(const Params& p, int r) {
+  if (kTiles == 1) return int(blockIdx.x);
+  const int c = (r & 1) ? int(gridDim.x) - 1 - int(blockIdx.x) : int(blockIdx.x);
+  const int w = r * int(gridDim.x) + c;
+  return w < p.n_items ? w : -1;
+}
+template <int kTiles>
+__device__ __forceinline__ Item make_item(const Params& p, int w, Walk& walk) {
+  Item it;
+  int block;
+  it.z = w % p.splits;
+  block_of(p, w / p.splits, block, it.kvh);
+  it.i0 = block * kTiles * p.tile_pos;
+  walk = make_walk(p, p.q_start + it.i0, p.q_start + min(it.i0 + kTiles * p.tile_pos, p.s_q) - 1);
+  it.j_lo = int((long long)walk.n * it.z / p.splits);
+  it.n_kv = int((long long)walk.n * (it.z + 1) / p.splits) - it.j_lo;
+  return it;
+}
+// The CTA's next work item with key tiles, from round r on; r becomes its round, or the number of rounds.
+template <int kTiles>
+__device__ __forceinline__ Item next_item(const Params& p, int& r, Walk& walk) {
+  Item it = {};
+  for (; r < rounds_of<kTiles>(p); ++r) {
+    const int w = item_of<kTiles>(p, r);
+    if (w < 0) continue;
+    it = make_item<kTiles>(p, w, walk);
+    if (it.n_kv > 0) break;
+  }
+  return it;
+}
+
 // Bits e of a 32-key word whose keys lie in [a, b] or below n (all relative to the word's first key).
 __device__ __forceinline__ uint32_t visible_bits(int a, int b, int n) {
   const uint32_t ge = a <= 0 ? 0xffffffffu : (a > 31 ? 0u : 0xffffffffu << a);
@@ -105,7 +157,7 @@ struct Cfg {
   static constexpr int kRel = kStages;
   static constexpr int kBarQ = 0, kBarKV = 1, kBarRel = kBarKV + kStages, kBarS = kBarRel + kRel,
                        kBarPSplit = kBarS + kTiles, kBarPLast = kBarPSplit + kTiles, kBarO = kBarPLast + kTiles,
-                       kBarDrain = kBarO + kTiles, kNumBars = kBarDrain + 1;
+                       kBarDrain = kBarO + kTiles, kBarQFree = kBarDrain + 1, kNumBars = kBarQFree + 1;
   static constexpr uint32_t kOffKV = kTiles * kTileBytes;
   static constexpr uint32_t kOffBars = kOffKV + kStages * kTileBytes;
   static constexpr uint32_t kSmem = 1024 + kOffBars + kNumBars * 8 + 16;
@@ -135,14 +187,6 @@ __global__ void __launch_bounds__(Cfg<kTiles>::kThreads, Cfg<kTiles>::kCtasPerSm
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int block, kvh;
-  block_of(p, blockIdx.x, block, kvh);
-  const int i0 = block * kTiles * p.tile_pos;  // first query position of the CTA
-  const Walk walk = make_walk(p, p.q_start + i0, p.q_start + min(i0 + kTiles * p.tile_pos, p.s_q) - 1);
-  // this CTA's share of the tile list
-  const int j_lo = int((long long)walk.n * blockIdx.z / gridDim.z);
-  const int n_kv = int((long long)walk.n * (blockIdx.z + 1) / gridDim.z) - j_lo;
-
   if (threadIdx.x == 0) {
     mbar_init(bar(C::kBarQ), 1);
     for (int s = 0; s < C::kStages; ++s) mbar_init(bar(C::kBarKV + s), 1);
@@ -154,6 +198,7 @@ __global__ void __launch_bounds__(Cfg<kTiles>::kThreads, Cfg<kTiles>::kCtasPerSm
       mbar_init(bar(C::kBarO + t), 1);
     }
     mbar_init(bar(C::kBarDrain), 1);
+    mbar_init(bar(C::kBarQFree), 1);
     *abort_flag = (*reinterpret_cast<volatile int*>(p.status) != 0) ? 1 : 0;
     fence_mbar_init();
   }
@@ -171,50 +216,60 @@ __global__ void __launch_bounds__(Cfg<kTiles>::kThreads, Cfg<kTiles>::kCtasPerSm
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const WaitCtx ctx{abort_flag, p.status};
-  const bool run = *abort_flag == 0 && n_kv > 0;  // uniform over the CTA
+  const bool run = *abort_flag == 0;  // uniform over the CTA
   if (warp < 4) {
     regs_dec<C::kRegsControl>();
     const uint32_t sq = sbase, skv = sbase + C::kOffKV;
     if (warp == 0 && run) {
       // ------------------------------------------------------------ TMA producer: Q, then K_0, V_0, K_1, V_1, ...
       const bool issuer = elect_one();
-      if (issuer) {
-        const uint32_t box = 64u * 2u * uint32_t(p.group * p.tile_pos);  // rows past group * tile_pos stay unused
-        mbar_expect_tx(bar(C::kBarQ), kTiles * 2 * box);
-        for (int t = 0; t < kTiles; ++t)
-          for (int hh = 0; hh < 2; ++hh)
-            tma_load_4d(sq + t * kTileBytes + hh * kHalfBytes, &tmap_q, bar(C::kBarQ), hh * 64, 0, i0 + t * p.tile_pos, kvh);
-      }
-      __syncwarp();
-      int it = 0;
+      int it = 0, q_loads = 0;  // ring items, work items so far
       bool ok = true;
-      for (int j = 0; ok && j < n_kv; ++j) {
-        const int key = walk.base(j_lo + j);
-        for (int kv = 0; kv < 2; ++kv, ++it) {
-          const int st = it % C::kStages;
-          if (it >= C::kStages) {
-            // the stage's previous item (it - kStages) is free once release e has completed: K_r (item 2r) after
-            // S(r), V_r (item 2r + 1) after S(r + 1)
-            const int e = (it - C::kStages + 1) / 2;
-            if (!__all_sync(0xffffffffu,
-                            mbar_wait(bar(C::kBarRel + e % C::kRel), uint32_t(e / C::kRel) & 1u, ctx, kStatusTimeoutKV))) {
-              ok = false;
-              break;
+      Walk walk;
+      int r = 0;
+      for (Item item = next_item<kTiles>(p, r, walk); ok && r < rounds_of<kTiles>(p); ++r, item = next_item<kTiles>(p, r, walk)) {
+        // Q is free once the last S of the item before is ready
+        if (q_loads > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(bar(C::kBarQFree), uint32_t(q_loads - 1) & 1u, ctx,
+                                                                    kStatusTimeoutQ))))
+          break;
+        if (issuer) {
+          const uint32_t box = 64u * 2u * uint32_t(p.group * p.tile_pos);  // rows past group * tile_pos stay unused
+          mbar_expect_tx(bar(C::kBarQ), kTiles * 2 * box);
+          for (int t = 0; t < kTiles; ++t)
+            for (int hh = 0; hh < 2; ++hh)
+              tma_load_4d(sq + t * kTileBytes + hh * kHalfBytes, &tmap_q, bar(C::kBarQ), hh * 64, 0,
+                          item.i0 + t * p.tile_pos, item.kvh);
+        }
+        __syncwarp();
+        ++q_loads;
+        for (int j = 0; ok && j < item.n_kv; ++j) {
+          const int key = walk.base(item.j_lo + j);
+          for (int kv = 0; kv < 2; ++kv, ++it) {
+            const int st = it % C::kStages;
+            if (it >= C::kStages) {
+              // the stage's previous item (it - kStages) is free once release e has completed: K_r (item 2r) after
+              // S(r), V_r (item 2r + 1) after S(r + 1); tiles are counted on across work items
+              const int e = (it - C::kStages + 1) / 2;
+              if (!__all_sync(0xffffffffu, mbar_wait(bar(C::kBarRel + e % C::kRel), uint32_t(e / C::kRel) & 1u, ctx,
+                                                     kStatusTimeoutKV))) {
+                ok = false;
+                break;
+              }
             }
+            if (issuer) {
+              const CUtensorMap* m = kv ? &tmap_v : &tmap_k;
+              const uint32_t dst = skv + st * kTileBytes;
+              mbar_expect_tx(bar(C::kBarKV + st), kTileBytes);
+              tma_load_3d(dst, m, bar(C::kBarKV + st), 0, key, item.kvh);
+              tma_load_3d(dst + kHalfBytes, m, bar(C::kBarKV + st), 64, key, item.kvh);
+            }
+            __syncwarp();
           }
-          if (issuer) {
-            const CUtensorMap* m = kv ? &tmap_v : &tmap_k;
-            const uint32_t dst = skv + st * kTileBytes;
-            mbar_expect_tx(bar(C::kBarKV + st), kTileBytes);
-            tma_load_3d(dst, m, bar(C::kBarKV + st), 0, key, kvh);
-            tma_load_3d(dst + kHalfBytes, m, bar(C::kBarKV + st), 64, key, kvh);
-          }
-          __syncwarp();
         }
       }
       // every issued copy must land before the CTA may exit
       if (issuer) {
-        drain_wait(bar(C::kBarQ), 0, p.status);
+        if (q_loads > 0) drain_wait(bar(C::kBarQ), uint32_t(q_loads - 1) & 1u, p.status);
         for (int st = 0; st < C::kStages; ++st) {
           const int cnt = it / C::kStages + (st < it % C::kStages ? 1 : 0);
           if (cnt > 0) drain_wait(bar(C::kBarKV + st), uint32_t(cnt - 1) & 1u, p.status);
@@ -236,8 +291,11 @@ __global__ void __launch_bounds__(Cfg<kTiles>::kThreads, Cfg<kTiles>::kCtasPerSm
       };
       auto col_o = [&](int t) { return tmem + 128u * uint32_t(kTiles + t); };
       auto col_p = [&](int t) { return tmem + 128u * uint32_t(t) + 64u; };
-      bool ok = wait_all(bar(C::kBarQ), 0, kStatusTimeoutQ) && wait_full(0);
-      if (ok) {
+      Walk walk, walk_next;
+      int r = 0, items = 0, jg = 0;  // round; work items and key tiles so far
+      Item item = next_item<kTiles>(p, r, walk);
+      bool ok = r < rounds_of<kTiles>(p);
+      if (ok && (ok = wait_all(bar(C::kBarQ), 0, kStatusTimeoutQ) && wait_full(0))) {
         tc_fence_after();
         for (int t = 0; t < kTiles; ++t) {
           if (issuer) issue_qk(tmem + 128u * t, sq + t * kTileBytes, skv);
@@ -245,45 +303,55 @@ __global__ void __launch_bounds__(Cfg<kTiles>::kThreads, Cfg<kTiles>::kCtasPerSm
           commit(C::kBarS + t);
         }
       }
-      for (int j = 0; ok && j < n_kv; ++j) {
-        const int it_v = 2 * j + 1, it_k = 2 * j + 2;
-        const bool next = j + 1 < n_kv;
-        if (!(ok = wait_full(it_v))) break;
-        const uint32_t sv = skv + (it_v % C::kStages) * kTileBytes;
-        const uint32_t sk = skv + (it_k % C::kStages) * kTileBytes;
-        const uint32_t ph = uint32_t(j) & 1u;
-        {
-          // keys behind the end of the run, inside its last tile: no row sees them, their V rows become zero
-          // (rows past s_kv already are: the TMA fill). The 128-byte swizzle permutes within a row only.
-          const int key = walk.base(j_lo + j);
-          const int from = walk.end(j_lo + j) - key, to = min(kBlockN, p.s_kv - key);
-          if (from < to) {
-            for (int c = 8 * from + lane; c < 8 * to; c += 32) {
-              st_shared_u4(sv + 16u * uint32_t(c), make_uint4(0, 0, 0, 0));
-              st_shared_u4(sv + kHalfBytes + 16u * uint32_t(c), make_uint4(0, 0, 0, 0));
+      while (ok) {
+        int r_next = r + 1;
+        const Item following = next_item<kTiles>(p, r_next, walk_next);
+        for (int j = 0; ok && j < item.n_kv; ++j, ++jg) {
+          const int it_v = 2 * jg + 1, it_k = 2 * jg + 2;
+          const bool last = j + 1 == item.n_kv;
+          const bool next = !last || r_next < rounds_of<kTiles>(p);
+          if (!(ok = wait_full(it_v))) break;
+          const uint32_t sv = skv + (it_v % C::kStages) * kTileBytes;
+          const uint32_t sk = skv + (it_k % C::kStages) * kTileBytes;
+          const uint32_t ph = uint32_t(jg) & 1u;
+          {
+            // keys behind the end of the run, inside its last tile: no row sees them, their V rows become zero
+            // (rows past s_kv already are: the TMA fill). The 128-byte swizzle permutes within a row only.
+            const int key = walk.base(item.j_lo + j);
+            const int from = walk.end(item.j_lo + j) - key, to = min(kBlockN, p.s_kv - key);
+            if (from < to) {
+              for (int c = 8 * from + lane; c < 8 * to; c += 32) {
+                st_shared_u4(sv + 16u * uint32_t(c), make_uint4(0, 0, 0, 0));
+                st_shared_u4(sv + kHalfBytes + 16u * uint32_t(c), make_uint4(0, 0, 0, 0));
+              }
+              fence_proxy_async();
+              __syncwarp();
             }
-            fence_proxy_async();
+          }
+          for (int t = 0; t < kTiles; ++t) {
+            if (!(ok = wait_all(bar(C::kBarPSplit + t), ph, kStatusTimeoutP))) break;
+            tc_fence_after();
+            if (issuer) issue_pv_steps<0, 2 * kSplitChunks>(col_o(t), col_p(t), sv, j > 0);
             __syncwarp();
+            if (!(ok = wait_all(bar(C::kBarPLast + t), ph, kStatusTimeoutP))) break;
+            tc_fence_after();
+            if (issuer) issue_pv_steps<2 * kSplitChunks, 8 - 2 * kSplitChunks>(col_o(t), col_p(t), sv, true);
+            __syncwarp();
+            if (last) commit(C::kBarO + t);
+            if (next) {
+              if (t == 0 && last && !(ok = wait_all(bar(C::kBarQ), uint32_t(items + 1) & 1u, kStatusTimeoutQ))) break;
+              if (t == 0 && !(ok = wait_full(it_k))) break;
+              if (issuer) issue_qk(tmem + 128u * t, sq + t * kTileBytes, sk);
+              __syncwarp();
+              commit(C::kBarS + t);
+            }
           }
         }
-        for (int t = 0; t < kTiles; ++t) {
-          if (!(ok = wait_all(bar(C::kBarPSplit + t), ph, kStatusTimeoutP))) break;
-          tc_fence_after();
-          if (issuer) issue_pv_steps<0, 2 * kSplitChunks>(col_o(t), col_p(t), sv, j > 0);
-          __syncwarp();
-          if (!(ok = wait_all(bar(C::kBarPLast + t), ph, kStatusTimeoutP))) break;
-          tc_fence_after();
-          if (issuer) issue_pv_steps<2 * kSplitChunks, 8 - 2 * kSplitChunks>(col_o(t), col_p(t), sv, true);
-          __syncwarp();
-          if (!next) {
-            commit(C::kBarO + t);
-          } else {
-            if (t == 0 && !(ok = wait_full(it_k))) break;
-            if (issuer) issue_qk(tmem + 128u * t, sq + t * kTileBytes, sk);
-            __syncwarp();
-            commit(C::kBarS + t);
-          }
-        }
+        if (r_next >= rounds_of<kTiles>(p)) break;
+        r = r_next;
+        item = following;
+        walk = walk_next;
+        ++items;
       }
       // every issued MMA must retire before TMEM is released
       if (issuer) {
@@ -306,175 +374,186 @@ __global__ void __launch_bounds__(Cfg<kTiles>::kThreads, Cfg<kTiles>::kCtasPerSm
     const int r_in = quad * 32 + lane;
     const int row_pos = r_in / p.group;              // packed row -> query position in the tile, head in the group
     const int row_head = r_in - row_pos * p.group;
-    const int it0 = i0 + t * p.tile_pos;             // the tile's first query
-    const int pos = p.q_start + it0 + row_pos;       // this row's key position
-    const int row_lo = pos - p.left, row_hi = min(pos + p.right, p.s_kv - 1);
-    const int row_ns = p.causal ? min(p.sinks, pos + 1) : p.sinks;
-    // what every row of the tile sees: keys below all_ns, keys of [all_lo, all_hi]
-    const int t_first = p.q_start + it0, t_last = t_first + p.tile_pos - 1;
-    const int all_lo = t_last - p.left, all_hi = min(t_first + p.right, p.s_kv - 1);
-    const int all_ns = p.causal ? min(p.sinks, t_first + 1) : p.sinks;
-    float m_run = -INFINITY;
-    uint64_t l_a = f2_pack(0.f, 0.f), l_b = f2_pack(0.f, 0.f);
     bool ok = run;
+    int jg = 0, items = 0;
+    for (int r = 0; ok && r < rounds_of<kTiles>(p); ++r) {
+      const int w = item_of<kTiles>(p, r);
+      if (w < 0) continue;
+      Walk walk;
+      const Item item = make_item<kTiles>(p, w, walk);
+      const int it0 = item.i0 + t * p.tile_pos;        // the tile's first query
+      const int pos = p.q_start + it0 + row_pos;       // this row's key position
+      const int row_lo = pos - p.left, row_hi = min(pos + p.right, p.s_kv - 1);
+      const int row_ns = p.causal ? min(p.sinks, pos + 1) : p.sinks;
+      // what every row of the tile sees: keys below all_ns, keys of [all_lo, all_hi]
+      const int t_first = p.q_start + it0, t_last = t_first + p.tile_pos - 1;
+      const int all_lo = t_last - p.left, all_hi = min(t_first + p.right, p.s_kv - 1);
+      const int all_ns = p.causal ? min(p.sinks, t_first + 1) : p.sinks;
+      float m_run = -INFINITY;
+      uint64_t l_a = f2_pack(0.f, 0.f), l_b = f2_pack(0.f, 0.f);
 
-    for (int j = 0; ok && j < n_kv; ++j) {
-      ok = __all_sync(0xffffffffu, mbar_wait(bar(C::kBarS + t), uint32_t(j) & 1u, ctx, kStatusTimeoutS));
-      if (!ok) break;
-      if (t == kTiles - 1 && quad == 0 && lane == 0) mbar_arrive(bar(C::kBarRel + j % C::kRel));
-      tc_fence_after();
-      const int key = walk.base(j_lo + j);
-      const bool first_run = j_lo + j < walk.a_tiles;
-      const bool masked = !(key + kBlockN <= all_ns ||
-                            (!first_run && key >= all_lo && key + kBlockN - 1 <= all_hi));
-      uint32_t sa[64], sb[64];
-      tmem_ld64_wait(tS, sa);
-      tmem_ld64_nowait(tS + 64, sb);
-      float s[128];
-#pragma unroll
-      for (int i = 0; i < 64; ++i) s[i] = __uint_as_float(sa[i]);
-      const int ma = first_run ? 1 << 20 : row_lo - key, mb = row_hi - key, mn = row_ns - key;
-      if (masked) {
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const uint32_t bits = visible_bits(ma - 32 * w, mb - 32 * w, mn - 32 * w);
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!((bits >> i) & 1u)) s[32 * w + i] = -INFINITY;
+      for (int j = 0; ok && j < item.n_kv; ++j, ++jg) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(C::kBarS + t), uint32_t(jg) & 1u, ctx, kStatusTimeoutS));
+        if (!ok) break;
+        if (t == kTiles - 1 && quad == 0 && lane == 0) {
+          mbar_arrive(bar(C::kBarRel + jg % C::kRel));
+          if (j + 1 == item.n_kv) mbar_arrive(bar(C::kBarQFree));  // every S of this item is done: Q may be replaced
         }
-      }
-      float mx0 = fmax3(s[0], s[1], s[2]), mx1 = fmax3(s[3], s[4], s[5]);
-      float mx2 = fmax3(s[6], s[7], s[8]), mx3 = fmax3(s[9], s[10], s[11]);
+        tc_fence_after();
+        const int key = walk.base(item.j_lo + j);
+        const bool first_run = item.j_lo + j < walk.a_tiles;
+        const bool masked = !(key + kBlockN <= all_ns ||
+                              (!first_run && key >= all_lo && key + kBlockN - 1 <= all_hi));
+        uint32_t sa[64], sb[64];
+        tmem_ld64_wait(tS, sa);
+        tmem_ld64_nowait(tS + 64, sb);
+        float s[128];
 #pragma unroll
-      for (int i = 12; i < 60; i += 8) {
-        mx0 = fmax3(mx0, s[i], s[i + 1]);
-        mx1 = fmax3(mx1, s[i + 2], s[i + 3]);
-        mx2 = fmax3(mx2, s[i + 4], s[i + 5]);
-        mx3 = fmax3(mx3, s[i + 6], s[i + 7]);
-      }
-      mx0 = fmax3(mx0, s[60], s[61]);
-      mx1 = fmax3(mx1, s[62], s[63]);
-      tmem_ld64_wait_on(sb);
+        for (int i = 0; i < 64; ++i) s[i] = __uint_as_float(sa[i]);
+        const int ma = first_run ? 1 << 20 : row_lo - key, mb = row_hi - key, mn = row_ns - key;
+        if (masked) {
 #pragma unroll
-      for (int i = 0; i < 64; ++i) s[64 + i] = __uint_as_float(sb[i]);
-      if (masked) {
+          for (int w = 0; w < 2; ++w) {
+            const uint32_t bits = visible_bits(ma - 32 * w, mb - 32 * w, mn - 32 * w);
 #pragma unroll
-        for (int w = 2; w < 4; ++w) {
-          const uint32_t bits = visible_bits(ma - 32 * w, mb - 32 * w, mn - 32 * w);
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!((bits >> i) & 1u)) s[32 * w + i] = -INFINITY;
-        }
-      }
-#pragma unroll
-      for (int i = 64; i < 120; i += 8) {
-        mx0 = fmax3(mx0, s[i], s[i + 1]);
-        mx1 = fmax3(mx1, s[i + 2], s[i + 3]);
-        mx2 = fmax3(mx2, s[i + 4], s[i + 5]);
-        mx3 = fmax3(mx3, s[i + 6], s[i + 7]);
-      }
-      mx0 = fmax3(mx0, s[120], s[121]);
-      mx1 = fmax3(mx1, s[122], s[123]);
-      mx2 = fmax3(mx2, s[124], s[125]);
-      mx3 = fmax3(mx3, s[126], s[127]);
-      const float m_new = fmaxf(m_run, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * c);
-      if (j == 0) {
-        m_run = m_new;
-      } else {
-        // rows whose running maximum grew by more than 2^8 (or from nothing) rescale O and l; O_t is quiescent
-        // here: S_t(j) ready implies every earlier P_t V has retired
-        const bool need = m_new > m_run + kRescaleThreshold;
-        if (__any_sync(0xffffffffu, need)) {
-          const float f = need ? ex2_approx(m_run - m_new) : 1.0f;
-          if (need) {
-            l_a = f2_fma(l_a, f2_pack(f, f), f2_pack(0.f, 0.f));
-            l_b = f2_fma(l_b, f2_pack(f, f), f2_pack(0.f, 0.f));
-            m_run = m_new;
+            for (int i = 0; i < 32; ++i)
+              if (!((bits >> i) & 1u)) s[32 * w + i] = -INFINITY;
           }
-#pragma unroll 1
-          for (int c16 = 0; c16 < 8; ++c16) {
-            uint32_t o[16];
-            tmem_ld16_wait(tO + c16 * 16, o);
+        }
+        float mx0 = fmax3(s[0], s[1], s[2]), mx1 = fmax3(s[3], s[4], s[5]);
+        float mx2 = fmax3(s[6], s[7], s[8]), mx3 = fmax3(s[9], s[10], s[11]);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_st16(tO + c16 * 16, o);
+        for (int i = 12; i < 60; i += 8) {
+          mx0 = fmax3(mx0, s[i], s[i + 1]);
+          mx1 = fmax3(mx1, s[i + 2], s[i + 3]);
+          mx2 = fmax3(mx2, s[i + 4], s[i + 5]);
+          mx3 = fmax3(mx3, s[i + 6], s[i + 7]);
+        }
+        mx0 = fmax3(mx0, s[60], s[61]);
+        mx1 = fmax3(mx1, s[62], s[63]);
+        tmem_ld64_wait_on(sb);
+#pragma unroll
+        for (int i = 0; i < 64; ++i) s[64 + i] = __uint_as_float(sb[i]);
+        if (masked) {
+#pragma unroll
+          for (int w = 2; w < 4; ++w) {
+            const uint32_t bits = visible_bits(ma - 32 * w, mb - 32 * w, mn - 32 * w);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!((bits >> i) & 1u)) s[32 * w + i] = -INFINITY;
           }
-          tmem_st_wait();
         }
-      }
-      // exponentials in four 32-key chunks, each stored as bf16 P as soon as it is done. A row that has seen no
-      // key yet keeps m_run = -inf: its weights are exp2(-inf - 0) = 0.
-      const float m_use = m_run == -INFINITY ? 0.f : m_run;
-      const uint64_t nm2 = f2_pack(-m_use, -m_use);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int e = 32 * k + 2 * i;
-          float x0, x1;
-          f2_unpack(f2_fma(f2_pack(s[e], s[e + 1]), c2, nm2), x0, x1);
-          s[e] = ex2_approx(x0);
-          s[e + 1] = ex2_approx(x1);
-          pk[i] = pack_bf16x2(s[e], s[e + 1]);
+        for (int i = 64; i < 120; i += 8) {
+          mx0 = fmax3(mx0, s[i], s[i + 1]);
+          mx1 = fmax3(mx1, s[i + 2], s[i + 3]);
+          mx2 = fmax3(mx2, s[i + 4], s[i + 5]);
+          mx3 = fmax3(mx3, s[i + 6], s[i + 7]);
         }
-        tmem_st16(tP + 16 * k, pk);
-        if (k == kSplitChunks - 1) {
-          tmem_st_wait();
-          tc_fence_before();
-          mbar_arrive(bar(C::kBarPSplit + t));
-        }
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(bar(C::kBarPLast + t));
-#pragma unroll
-      for (int i = 0; i < 128; i += 4) {
-        l_a = f2_add(l_a, f2_pack(s[i], s[i + 1]));
-        l_b = f2_add(l_b, f2_pack(s[i + 2], s[i + 3]));
-      }
-    }
-    float la0, la1, lb0, lb1;
-    f2_unpack(l_a, la0, la1);
-    f2_unpack(l_b, lb0, lb1);
-    const float l_run = (la0 + la1) + (lb0 + lb1);
-    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(C::kBarO + t), 0, ctx, kStatusTimeoutO));
-    // a CTA without keys writes its zeros too; an aborted one writes nothing
-    if (ok || (n_kv == 0 && *abort_flag == 0)) {
-      tc_fence_after();
-      const int i = it0 + row_pos;
-      const int head = kvh * p.group + row_head;
-      const bool valid = row_pos < p.tile_pos && i < p.s_q;
-      const bool none = n_kv == 0 || l_run == 0.f;
-      const float inv = 1.0f / l_run;
-      const long long ri = valid ? i : 0;
-      __nv_bfloat16* dst = p.o + (ri / p.o_rank_rows) * p.o_rank_stride + (long long)head * p.o_head_stride +
-                           (ri % p.o_rank_rows) * p.o_row_stride;
-      const long long part = ((long long)blockIdx.z * p.n_heads + head) * p.s_q + ri;
-#pragma unroll
-      for (int c4 = 0; c4 < 4; ++c4) {
-        uint32_t o[32];
-        tmem_ld32_wait(tO + c4 * 32, o);
-        if (!valid) continue;
-        if (p.part_o != nullptr) {
-          float4* d = reinterpret_cast<float4*>(p.part_o + part * 128 + c4 * 32);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            d[e] = none ? make_float4(0.f, 0.f, 0.f, 0.f)
-                        : make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
-                                      __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+        mx0 = fmax3(mx0, s[120], s[121]);
+        mx1 = fmax3(mx1, s[122], s[123]);
+        mx2 = fmax3(mx2, s[124], s[125]);
+        mx3 = fmax3(mx3, s[126], s[127]);
+        const float m_new = fmaxf(m_run, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * c);
+        if (j == 0) {
+          m_run = m_new;
         } else {
-          uint32_t w[16];
+          // rows whose running maximum grew by more than 2^8 (or from nothing) rescale O and l; O_t is quiescent
+          // here: S_t(j) ready implies every earlier P_t V has retired
+          const bool need = m_new > m_run + kRescaleThreshold;
+          if (__any_sync(0xffffffffu, need)) {
+            const float f = need ? ex2_approx(m_run - m_new) : 1.0f;
+            if (need) {
+              l_a = f2_fma(l_a, f2_pack(f, f), f2_pack(0.f, 0.f));
+              l_b = f2_fma(l_b, f2_pack(f, f), f2_pack(0.f, 0.f));
+              m_run = m_new;
+            }
+#pragma unroll 1
+            for (int c16 = 0; c16 < 8; ++c16) {
+              uint32_t o[16];
+              tmem_ld16_wait(tO + c16 * 16, o);
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            w[e] = none ? 0u : pack_bf16x2(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
-          uint4* d = reinterpret_cast<uint4*>(dst + c4 * 32);
+              for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_st16(tO + c16 * 16, o);
+            }
+            tmem_st_wait();
+          }
+        }
+        // exponentials in four 32-key chunks, each stored as bf16 P as soon as it is done. A row that has seen no
+        // key yet keeps m_run = -inf: its weights are exp2(-inf - 0) = 0.
+        const float m_use = m_run == -INFINITY ? 0.f : m_run;
+        const uint64_t nm2 = f2_pack(-m_use, -m_use);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) d[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+        for (int k = 0; k < 4; ++k) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int e = 32 * k + 2 * i;
+            float x0, x1;
+            f2_unpack(f2_fma(f2_pack(s[e], s[e + 1]), c2, nm2), x0, x1);
+            s[e] = ex2_approx(x0);
+            s[e + 1] = ex2_approx(x1);
+            pk[i] = pack_bf16x2(s[e], s[e + 1]);
+          }
+          tmem_st16(tP + 16 * k, pk);
+          if (k == kSplitChunks - 1) {
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(bar(C::kBarPSplit + t));
+          }
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(bar(C::kBarPLast + t));
+#pragma unroll
+        for (int i = 0; i < 128; i += 4) {
+          l_a = f2_add(l_a, f2_pack(s[i], s[i + 1]));
+          l_b = f2_add(l_b, f2_pack(s[i + 2], s[i + 3]));
         }
       }
-      if (valid && p.part_ml != nullptr) {
-        reinterpret_cast<float2*>(p.part_ml)[part] = make_float2(m_run, none ? 0.f : l_run);
+      float la0, la1, lb0, lb1;
+      f2_unpack(l_a, la0, la1);
+      f2_unpack(l_b, lb0, lb1);
+      const float l_run = (la0 + la1) + (lb0 + lb1);
+      if (ok && item.n_kv > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(C::kBarO + t), uint32_t(items) & 1u, ctx, kStatusTimeoutO));
+        ++items;
+      }
+      // an item without keys writes its zeros too; an aborted one writes nothing
+      if (ok) {
+        tc_fence_after();
+        const int i = it0 + row_pos;
+        const int head = item.kvh * p.group + row_head;
+        const bool valid = row_pos < p.tile_pos && i < p.s_q;
+        const bool none = item.n_kv == 0 || l_run == 0.f;
+        const float inv = 1.0f / l_run;
+        const long long ri = valid ? i : 0;
+        __nv_bfloat16* dst = p.o + (ri / p.o_rank_rows) * p.o_rank_stride + (long long)head * p.o_head_stride +
+                             (ri % p.o_rank_rows) * p.o_row_stride;
+        const long long part = ((long long)item.z * p.n_heads + head) * p.s_q + ri;
+#pragma unroll
+        for (int c4 = 0; c4 < 4; ++c4) {
+          uint32_t o[32];
+          tmem_ld32_wait(tO + c4 * 32, o);
+          if (!valid) continue;
+          if (p.part_o != nullptr) {
+            float4* d = reinterpret_cast<float4*>(p.part_o + part * 128 + c4 * 32);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              d[e] = none ? make_float4(0.f, 0.f, 0.f, 0.f)
+                          : make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
+                                        __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+          } else {
+            uint32_t w[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              w[e] = none ? 0u : pack_bf16x2(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+            uint4* d = reinterpret_cast<uint4*>(dst + c4 * 32);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+          }
+        }
+        if (valid && p.part_ml != nullptr) reinterpret_cast<float2*>(p.part_ml)[part] = make_float2(m_run, none ? 0.f : l_run);
       }
     }
   }
@@ -722,7 +801,7 @@ struct Plan {
   int tile_pos; // query positions per Q tile
   int blocks;    // blocks of queries per key head
   int first_mid, n_mid, heads_turn;  // their order (Params)
-  int splits;
+  int splits, n_items, ctas;
   int token;     // cluster size of token_kernel, or 0: window_kernel
 };
 
@@ -743,9 +822,10 @@ static int make_plan(const Shape& s, int64_t splits_asked, Plan& pl) {
   const int64_t left = s.left < 0 || s.left > kMaxPos ? kMaxPos : s.left;
   const int64_t right = s.causal ? 0 : (s.right < 0 || s.right > kMaxPos ? kMaxPos : s.right);
   if (ctas > (1ll << 30)) return H3_ERR_SHAPE;
-  // Blocks of the middle (whole windows) first, the shorter ones at the ends last, longest first: the last round of CTAs
-  // is short. Causal without a left bound, 28 heads x 8192: 515 us in ascending order, 481 so; 56 x 2048: 98 and 87; two-sided
-  // windows measure the same either way. Heads turn while the K and V of all of them stay in half of the L2.
+  // Blocks of the middle (whole windows) first, the shorter ones at the ends last, longest first, so that the CTAs' shares
+  // even out (Params, item_of). Heads turn while the keys that all of them look at fit the L2 twice: causal without a left
+  // bound, 28 heads x 8192 (117 MB): 525 us head by head, 478 in turn; 7 x 42000 (150 MB): 2749 and 2558; but 56 x 20000
+  // (573 MB): 5.63 ms and 6.14.
   const int64_t p0 = s.q_start;
   int64_t a = left >= kMaxPos ? blocks : (std::max<int64_t>(left - p0, 0) + per_cta - 1) / per_cta;
   a = std::min(a, blocks);
@@ -754,18 +834,22 @@ static int make_plan(const Shape& s, int64_t splits_asked, Plan& pl) {
   pl.blocks = (int)blocks;
   pl.first_mid = (int)a;
   pl.n_mid = (int)(b - a);
-  pl.heads_turn = s.n_kv_heads * s.s_kv * 512 <= (64ll << 20);
   const int64_t span = std::min(s.s_kv, left + right + per_cta) + std::min(s.sinks, s.s_kv);
+  pl.heads_turn = s.n_kv_heads * std::min(span, s.s_kv) * 512 <= (256ll << 20);
   const int64_t key_tiles = (std::min(span, s.s_kv) + kBlockN - 1) / kBlockN;
   pl.token = 0;
   if (splits_asked == 0 && s.s_q == 1 && group <= 4 && s.n_kv_heads * kTokenMaxCluster >= sms) {
     pl.token = (int)std::max<int64_t>(1, std::min<int64_t>(kTokenMaxCluster, key_tiles));
-    pl.splits = 1;
+    pl.splits = pl.n_items = pl.ctas = 1;
     return H3_OK;
   }
   int64_t splits = splits_asked;
   if (splits == 0) splits = std::min(slots / std::max<int64_t>(ctas, 1), key_tiles / 2);
   pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(splits, kMaxSplits));
+  if (ctas * pl.splits > (1ll << 30)) return H3_ERR_SHAPE;
+  pl.n_items = (int)ctas * pl.splits;
+  // two tiles: a CTA per SM walks the items; one tile: a CTA per item (few rows: there are hardly more than fit)
+  pl.ctas = pl.tiles == 2 ? std::min(pl.n_items, sms) : pl.n_items;
   return H3_OK;
 }
 
@@ -792,7 +876,7 @@ static int make_q_map(CUtensorMap* map, const void* q, const Shape& s, int64_t h
 
 template <int kTiles>
 static int launch(cudaStream_t st, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const Params& p,
-                  const Plan& pl, unsigned kv_heads) {
+                  const Plan& pl) {
   using C = Cfg<kTiles>;
   auto* kern = window_kernel<kTiles>;
   // setmaxnreg draws on the registers the CTA is launched with: the split must fit them
@@ -803,7 +887,7 @@ static int launch(cudaStream_t st, const CUtensorMap& q, const CUtensorMap& k, c
   if (regs * C::kThreads < 128 * C::kRegsControl + 128 * kTiles * C::kRegsSoftmax) return H3_ERR_UNSUPPORTED;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem) != cudaSuccess)
     return H3_ERR_LAUNCH;
-  kern<<<dim3((unsigned)pl.blocks * kv_heads, 1, (unsigned)pl.splits), C::kThreads, C::kSmem, st>>>(q, k, v, p);
+  kern<<<(unsigned)pl.ctas, C::kThreads, C::kSmem, st>>>(q, k, v, p);
   return cudaGetLastError() == cudaSuccess ? H3_OK : H3_ERR_LAUNCH;
 }
 
@@ -866,6 +950,9 @@ extern "C" int h3_window_attn(const void* q, const void* k, const void* v, void*
   p.n_mid = pl.n_mid;
   p.kv_heads = (int)n_kv_heads;
   p.heads_turn = pl.heads_turn;
+  p.splits = pl.splits;
+  p.n_items = pl.n_items;
+  p.rounds = (pl.n_items + pl.ctas - 1) / pl.ctas;
   p.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
   p.o = reinterpret_cast<__nv_bfloat16*>(o);
   p.o_rank_rows = o_rank_rows;
@@ -900,8 +987,7 @@ extern "C" int h3_window_attn(const void* q, const void* k, const void* v, void*
   if ((rc = make_q_map(&mq, q, s, q_head_stride, q_row_stride, pl.tile_pos)) != H3_OK) return rc;
   if ((rc = make_head_map(&mk, k, s_kv, n_kv_heads, kv_row_stride, kvhs)) != H3_OK) return rc;
   if ((rc = make_head_map(&mv, v, s_kv, n_kv_heads, kv_row_stride, kvhs)) != H3_OK) return rc;
-  rc = pl.tiles == 2 ? launch<2>(st, mq, mk, mv, p, pl, (unsigned)n_kv_heads)
-                     : launch<1>(st, mq, mk, mv, p, pl, (unsigned)n_kv_heads);
+  rc = pl.tiles == 2 ? launch<2>(st, mq, mk, mv, p, pl) : launch<1>(st, mq, mk, mv, p, pl);
   if (rc != H3_OK || pl.splits == 1) return rc;
   return launch_dependent(join_kernel, dim3((unsigned)(n_heads * s_q)), 32 * kJoinWarps, 0, st, p, pl.splits);
 }
