@@ -176,11 +176,11 @@ struct PackOut {
   const unsigned long long* rank_base;  // or one buffer per destination rank (peer memory)
   long long tensor_stride, row_offset;
   int heads_per_rank;
-  unsigned rank_magic;  // ceil(2^32 / heads_per_rank): h / heads_per_rank = h * magic >> 32 for h < 2^16 (one rank: 0)
+  unsigned rank_magic;  // ceil(2^32 / heads_per_rank): h / heads_per_rank = h * magic >> 32 for h < 2^16, from 2 heads a rank
 };
 template <int kTensor>
 __device__ __forceinline__ __nv_bfloat16* pack_row(const PackOut& o, int h, long long tok) {
-  const int r = int(__umulhi((unsigned)h, o.rank_magic)), hl = h - r * o.heads_per_rank;
+  const int r = o.heads_per_rank == 1 ? h : int(__umulhi((unsigned)h, o.rank_magic)), hl = h - r * o.heads_per_rank;
   return o.rank_base != nullptr
              ? reinterpret_cast<__nv_bfloat16*>(o.rank_base[r]) + kTensor * o.tensor_stride +
                    (long long)hl * o.head_stride + (o.row_offset + tok) * kHeadDim
@@ -311,7 +311,7 @@ static int pack_impl(const void* q, const void* k, const void* v, int64_t in_row
   in.w[1] = reinterpret_cast<const __nv_bfloat16*>(k_weight);
   in.eps = eps;
   o.heads_per_rank = (int)heads_per_rank;
-  o.rank_magic = heads_per_rank == n_heads ? 0u : (unsigned)(((1ull << 32) + heads_per_rank - 1) / heads_per_rank);
+  o.rank_magic = (unsigned)(((1ull << 32) + heads_per_rank - 1) / heads_per_rank);
   int parts = 1, part_heads = 1, rc;
   if ((rc = head_parts(s_l, n_heads, parts, part_heads)) != H3_OK) return rc;
   pack_axes_kernel<<<grid_for(s_l * parts, kWarps, 1 << 20), 32 * kWarps, 0, reinterpret_cast<cudaStream_t>(stream)>>>(

@@ -159,8 +159,15 @@ def _on(index: int):
 
 
 def _status_ptr(index: int) -> int:
+    """Address of the status word, made before the first launch that hands it out: zeroed on its stream, and not
+    inside a graph capture, whose pool would own it."""
     st = _status.get(index)
-    return (st if st is not None else status_word(torch.device("cuda", index))).data_ptr()
+    if st is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise H3Error("call status_word() once before the first graph capture on this device")
+        st = status_word(torch.device("cuda", index))
+        torch.cuda.current_stream().synchronize()
+    return st.data_ptr()
 
 
 def status_word(device=None) -> torch.Tensor:
@@ -454,13 +461,15 @@ def attention_peer(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o_local: t
 def _pack_args(q, k, v, rope, q_weight, k_weight):
     """Checks shared by the pack entry points; returns (q2, k2, v2, tokens, heads, rope_ptr,
     rope_row_stride, [q_weight_ptr, k_weight_ptr])."""
+    rows = []
     for n, t in (("q", q), ("k", k), ("v", v)):
         _cuda(t, n)
         if t.dim() == 3:
             t = t.reshape(t.shape[0], -1)
         if t.dim() != 2 or t.stride(-1) != 1:
             raise H3Error(f"{n} must be [tokens, heads*128] with a contiguous last dim")
-    q2, k2, v2 = (t.reshape(t.shape[0], -1) if t.dim() == 3 else t for t in (q, k, v))
+        rows.append(t)
+    q2, k2, v2 = rows
     sl, hd = q2.shape
     if hd % D or k2.shape != q2.shape or v2.shape != q2.shape:
         raise H3Error("q, k, v must share shape [tokens, heads*128]")

@@ -208,3 +208,12 @@ def test_launch_order_of_query_blocks():
                     for h in range(heads):
                         far = [max(first - b, b - first - mid + 1, 0) for b, kvh in got if kvh == h]
                         assert far == sorted(far)
+
+
+def test_rank_of_a_head_by_multiplication():
+    """h // heads_per_rank as the pack computes it (2 heads a rank and more), for every head it takes."""
+    for per in list(range(2, 300)) + [1000, 4095, 32768, 65535]:
+        magic = (2 ** 32 + per - 1) // per
+        assert magic < 2 ** 32
+        for h in {0, 1, per - 1, per, min(per + 1, 65535), min(2 * per - 1, 65535), 65534, 65535 - 65535 % per, 65535}:
+            assert h * magic >> 32 == h // per

@@ -122,7 +122,8 @@ def _pack64(x, w, rp, eps, s, H, turned=True):
 
 
 @pytest.mark.parametrize("s,H,world,axes,real", [(1, 1, 1, 1, False), (1, 56, 2, 3, False), (67, 8, 4, 3, True),
-                                                 (333, 56, 8, 4, False), (2600, 7, 1, 2, True)])
+                                                 (333, 56, 8, 4, False), (2600, 7, 1, 2, True), (40, 8, 8, 3, False),
+                                                 (20, 21, 7, 3, False), (9, 300, 4, 1, False)])
 def test_pack_with_positions(cuda_dev, s, H, world, axes, real):
     import h3attn as O
     q, k, v = _rand((s, 3 * H * D), 10, cuda_dev).split(H * D, -1)
