@@ -262,3 +262,12 @@ def test_refusals(cuda_dev):
     for f in bad:
         with pytest.raises(O.H3Error):
             f()
+
+
+def test_status_word_is_not_made_inside_a_capture(cuda_dev, monkeypatch):
+    import h3attn as O
+    monkeypatch.setattr(O, "_status", {})
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    q = _rand((2, 3, D), 40, cuda_dev)
+    with pytest.raises(O.H3Error):
+        O.window_attention(q, q, q, 1, 1)
