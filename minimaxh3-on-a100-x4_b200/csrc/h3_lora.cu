@@ -47,21 +47,30 @@ __device__ __forceinline__ int adapter_of(const Adapters& ad, int m, int r) {
 }
 
 // ---------------------------------------------------------------- tile path: T = s A x
-constexpr int kLowerStages = 3;
-constexpr int kPass = 2;  // chunks per pass over k: 16 KB of x and 2 x 8 KB of A per stage, two CTAs per SM
+// k is summed in kQuarters parts, each on its own, and the parts are added in ascending order. With few tiles of rows a
+// cluster of kQuarters CTAs takes one part each (kCluster = 4) and the parts meet in distributed shared memory; with many, one
+// CTA takes them one after the other (kCluster = 1). Both give the same bits, so a row's T does not depend on the
+// call's length. One CTA per SM. 42000 rows of 7168: 99 us = 6.1 TB/s; whole calls of 1000 rows, 7168 -> 5376: 98 us with
+// one CTA per tile over all of k, 82 so; 65 rows of 5376 -> 21504: 86 and 77.
+constexpr int kQuarters = 4;
+constexpr int kLowerStages = 6;
+constexpr int kPass = 2;  // chunks per pass over k: 16 KB of x and 2 x 8 KB of A per stage
 constexpr uint32_t kChunkBytes = 64u * 64u * 2u;
 constexpr uint32_t kLowerStage = kTileBytes + kPass * kChunkBytes;
+constexpr int kSumRow = 64 * kPass + 4;  // floats of a row of the cluster's sums (padded against bank conflicts)
+static_assert(128 * kSumRow * 4 <= kLowerStages * kLowerStage, "the sums reuse the ring");
 struct LowerSmem {
   uint32_t own[kMaxChunks / 32], both[kMaxChunks / 32];  // chunks in use: these 128 rows, the block of 256
   uint16_t list[kMaxChunks];
   int count;
-  uint64_t bars[2 * kLowerStages + 5];
+  uint64_t bars[2 * kLowerStages + 3];
   uint32_t tmem;
   int abort;
 };
 constexpr uint32_t kLowerSmem = 1024 + kLowerStages * kLowerStage + sizeof(LowerSmem);
 
-__global__ void __launch_bounds__(192, 2)
+template <int kCluster>
+__global__ void __launch_bounds__(192, 1)
     lower_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_a,
                  const Adapters ad, __nv_bfloat16* low, int* chunks, int chunk_stride, int m, int n_kb, int kc_blocks,
                  int* status) {
@@ -70,10 +79,13 @@ __global__ void __launch_bounds__(192, 2)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
   LowerSmem& sh = *reinterpret_cast<LowerSmem*>(smem + kLowerStages * kLowerStage);
-  enum { kF = 0, kE = kLowerStages, kAccF = 2 * kLowerStages, kAccE = kAccF + 2, kD = kAccE + 2 };
+  enum { kF = 0, kE = kLowerStages, kAccF = 2 * kLowerStages, kAccE = kAccF + 1, kD = kAccE + 1 };
   auto bar = [&](int i) { return smem_u32(&sh.bars[i]); };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int m0 = blockIdx.x * 128;
+  const int tile = blockIdx.x / kCluster, m0 = tile * 128;
+  const int rank = kCluster > 1 ? int(cluster_ctarank()) : 0;
+  const int q_begin = kCluster > 1 ? rank : 0, q_end = kCluster > 1 ? rank + 1 : kQuarters;  // this CTA's parts of k
+  auto part = [&](int q) { return n_kb * q / kQuarters; };                                  // first k-block of part q
 
   for (int i = threadIdx.x; i < kMaxChunks / 32; i += 192) sh.own[i] = sh.both[i] = 0;
   if (threadIdx.x == 0) {
@@ -81,16 +93,14 @@ __global__ void __launch_bounds__(192, 2)
       mbar_init(bar(kF + s), 1);
       mbar_init(bar(kE + s), 1);
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(bar(kAccF + b), 1);
-      mbar_init(bar(kAccE + b), 4);
-    }
+    mbar_init(bar(kAccF), 1);
+    mbar_init(bar(kAccE), 4);
     mbar_init(bar(kD), 1);
     sh.abort = *reinterpret_cast<volatile int*>(status) != 0 ? 1 : 0;
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(&sh.tmem), 256);
+    tmem_alloc(smem_u32(&sh.tmem), 512);  // part q, chunk i of the pass at 64 (kPass q + i)
     tmem_relinquish();
   }
   __syncthreads();
@@ -108,7 +118,7 @@ __global__ void __launch_bounds__(192, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 2 || (warp == 3 && (blockIdx.x & 1) == 0)) {
+  if (warp == 2 || (warp == 3 && (tile & 1) == 0 && rank == 0)) {
     // ascending lists: this tile's in shared memory, the block's (its first tile writes it) in global memory
     const uint32_t word = warp == 2 ? sh.own[lane] : sh.both[lane];
     int at = __popc(word);
@@ -117,7 +127,7 @@ __global__ void __launch_bounds__(192, 2)
       const int up = __shfl_up_sync(0xffffffffu, at, o);
       if (lane >= o) at += up;
     }
-    int* out = chunks + (long long)(blockIdx.x >> 1) * chunk_stride;
+    int* out = chunks + (long long)(tile >> 1) * chunk_stride;
     if (lane == 31) {
       if (warp == 2)
         sh.count = at;
@@ -140,13 +150,27 @@ __global__ void __launch_bounds__(192, 2)
   const bool run = sh.abort == 0 && count > 0;
   const int passes = (count + kPass - 1) / kPass;
 
-  if (warp == 0 && run) {
-    const bool issuer = elect_one();
-    int it = 0;
-    bool ok = true;
-    for (int ps = 0; ok && ps < passes; ++ps) {
-      const int nc = min(kPass, count - ps * kPass);
-      for (int kb = 0; kb < n_kb; ++kb, ++it) {
+  const bool issuer = warp < 2 && elect_one();
+  const int quad = warp & 3;
+  const uint32_t lane_off = uint32_t(quad * 32) << 16;
+  float* sums = reinterpret_cast<float*>(smem);  // kCluster > 1: [128 rows][kSumRow] of this CTA's part, between passes
+  int it = 0;                                    // ring items so far
+  bool ok = run;
+  // Where a row's T goes: 8 stacked columns from `col` on, if they are its adapter's.
+  auto put = [&](int row, int col, const float (&v)[8]) {
+    const int a = adapter_of(ad, m, row);
+    if (a < 0 || col < a * ad.rank || col >= (a + 1) * ad.rank) return;
+    const float scale = ad.scale[a];
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(v[2 * e] * scale, v[2 * e + 1] * scale);
+    *reinterpret_cast<uint4*>(low + (long long)row * ad.rank + (col - a * ad.rank)) = make_uint4(w[0], w[1], w[2], w[3]);
+  };
+
+  for (int ps = 0; ps < passes; ++ps) {
+    const int nc = min(kPass, count - ps * kPass);
+    if (warp == 0) {
+      for (int kb = part(q_begin); ok && kb < part(q_end); ++kb, ++it) {
         const int st = it % kLowerStages;
         if (it >= kLowerStages &&
             !(ok = __all_sync(0xffffffffu, mbar_wait(bar(kE + st), uint32_t(it / kLowerStages - 1) & 1u, ctx,
@@ -162,91 +186,103 @@ __global__ void __launch_bounds__(192, 2)
         }
         __syncwarp();
       }
-    }
-    if (issuer)
-      for (int st = 0; st < kLowerStages; ++st) {
-        const int cnt = it / kLowerStages + (st < it % kLowerStages ? 1 : 0);
-        if (cnt > 0) drain_wait_cluster(bar(kF + st), uint32_t(cnt - 1) & 1u, status);
-      }
-    __syncwarp();
-  } else if (warp == 1 && run) {
-    const bool issuer = elect_one();
-    constexpr uint32_t idesc = idesc_bf16_f32(128, 64, 0, 0);
-    int it = 0;
-    bool ok = true;
-    for (int ps = 0; ok && ps < passes; ++ps) {
-      const int b = ps & 1, nc = min(kPass, count - ps * kPass);
-      if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar(kAccE + b), (uint32_t(ps >> 1) & 1u) ^ 1u, ctx, kStatusTimeoutO))))
-        break;
+    } else if (warp == 1) {
+      constexpr uint32_t idesc = idesc_bf16_f32(128, 64, 0, 0);
+      if (ok && ps > 0)  // the pass before has been read out of the accumulators
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(kAccE), uint32_t(ps - 1) & 1u, ctx, kStatusTimeoutO));
       tc_fence_after();
-      for (int kb = 0; kb < n_kb; ++kb, ++it) {
-        const int st = it % kLowerStages;
-        if (!(ok = __all_sync(0xffffffffu,
-                              mbar_wait(bar(kF + st), uint32_t(it / kLowerStages) & 1u, ctx, kStatusTimeoutKV))))
-          break;
-        tc_fence_after();
-        if (issuer) {
-          const uint32_t x = sbase + st * kLowerStage;
-          for (int i = 0; i < nc; ++i)
-            for (int ks = 0; ks < 4; ++ks)
-              mma_ss(tmem + 128u * b + 64u * i, smem_desc_sw128(x + 32u * ks, 16, 1024),
-                     smem_desc_sw128(x + kTileBytes + i * kChunkBytes + 32u * ks, 16, 1024), idesc,
-                     kb > 0 || ks > 0 ? 1u : 0u);
-          mma_commit(bar(kE + st));
+      for (int q = q_begin; q < q_end; ++q)
+        for (int kb = part(q); ok && kb < part(q + 1); ++kb, ++it) {
+          const int st = it % kLowerStages;
+          if (!(ok = __all_sync(0xffffffffu,
+                                mbar_wait(bar(kF + st), uint32_t(it / kLowerStages) & 1u, ctx, kStatusTimeoutKV))))
+            break;
+          tc_fence_after();
+          if (issuer) {
+            const uint32_t x = sbase + st * kLowerStage;
+            for (int i = 0; i < nc; ++i)
+              for (int ks = 0; ks < 4; ++ks)
+                mma_ss(tmem + 64u * uint32_t(kPass * q + i), smem_desc_sw128(x + 32u * ks, 16, 1024),
+                       smem_desc_sw128(x + kTileBytes + i * kChunkBytes + 32u * ks, 16, 1024), idesc,
+                       kb > part(q) || ks > 0 ? 1u : 0u);
+            mma_commit(bar(kE + st));
+          }
+          __syncwarp();
         }
-        __syncwarp();
-      }
-      if (ok && issuer) mma_commit(bar(kAccF + b));
+      if (ok && issuer) mma_commit(bar(kAccF));
       __syncwarp();
-    }
-    if (issuer) {
-      mma_commit(bar(kD));
-      drain_wait_cluster(bar(kD), 0, status);
-    }
-    __syncwarp();
-  } else if (warp >= 2 && run) {
-    const int quad = warp & 3;
-    const uint32_t lane_off = uint32_t(quad * 32) << 16;
-    const int row = m0 + quad * 32 + lane;
-    const int a = adapter_of(ad, m, row);
-    const float scale = a >= 0 ? ad.scale[a] : 0.f;
-    const int lo = a >= 0 ? a * ad.rank : 0, hi = a >= 0 ? lo + ad.rank : 0;  // the row's stacked columns
-    bool ok = true;
-    for (int ps = 0; ok && ps < passes; ++ps) {
-      const int b = ps & 1, nc = min(kPass, count - ps * kPass);
-      ok = __all_sync(0xffffffffu, mbar_wait(bar(kAccF + b), uint32_t(ps >> 1) & 1u, ctx, kStatusTimeoutS));
-      if (!ok) break;
+    } else {
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(kAccF), uint32_t(ps) & 1u, ctx, kStatusTimeoutS));
       tc_fence_after();
-      for (int i = 0; i < nc; ++i) {
-        const int first = 64 * sh.list[ps * kPass + i];
+      const int r_in = quad * 32 + lane;
+      for (int i = 0; i < nc; ++i)
 #pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-          uint32_t r[16];
-          tmem_ld16_wait(tmem + lane_off + 128u * b + 64u * i + 16u * q, r);
+        for (int c = 0; c < 4; ++c) {
+          float v[16];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int col = first + 16 * q + 8 * h;
-            if (col >= lo && col < hi) {
-              uint32_t w[4];
+          for (int e = 0; e < 16; ++e) v[e] = 0.f;
+          for (int q = q_begin; q < q_end; ++q) {
+            if (!ok || part(q) == part(q + 1)) continue;
+            uint32_t r[16];
+            tmem_ld16_wait(tmem + lane_off + 64u * uint32_t(kPass * q + i) + 16u * c, r);
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                w[e] = pack_bf16x2(__uint_as_float(r[8 * h + 2 * e]) * scale,
-                                   __uint_as_float(r[8 * h + 2 * e + 1]) * scale);
-              *reinterpret_cast<uint4*>(low + (long long)row * ad.rank + (col - lo)) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+            for (int e = 0; e < 16; ++e) v[e] += __uint_as_float(r[e]);
+          }
+          if constexpr (kCluster > 1) {
+            float4* d = reinterpret_cast<float4*>(sums + r_in * kSumRow + 64 * i + 16 * c);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+          } else if (ok) {
+            const int col = 64 * sh.list[ps * kPass + i] + 16 * c;
+            const float lo[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
+            const float hi[8] = {v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15]};
+            put(m0 + r_in, col, lo);
+            put(m0 + r_in, col + 8, hi);
           }
         }
-      }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(kAccE + b));
+      if (lane == 0) mbar_arrive(bar(kAccE));
+    }
+    if constexpr (kCluster > 1) {
+      // the ring is idle: every MMA of the pass has retired (kAccF), and nothing was loaded beyond it. This CTA adds the
+      // parts of its 32 rows.
+      __syncthreads();
+      cluster_sync_all();
+      constexpr int kRows = 128 / kCluster;
+      for (int i = threadIdx.x; i < kRows * 8 * nc; i += 192) {
+        const int r_in = kRows * rank + i / (8 * nc), piece = i % (8 * nc);
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 0.f;
+        const uint32_t from = smem_u32(sums + r_in * kSumRow + 8 * piece);
+#pragma unroll
+        for (int q = 0; q < kCluster; ++q) {
+          const uint32_t at = mapa_shared(from, q);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += ld_cluster_f32(at + 4u * e);
+        }
+        if (sh.abort == 0) put(m0 + r_in, 64 * sh.list[ps * kPass + piece / 8] + 8 * (piece % 8), v);
+      }
+      cluster_sync_all();   // the sums have been read: the ring may be filled again
+      fence_proxy_async();  // by the async proxy
     }
   }
+  if (warp == 0 && issuer) {
+    for (int st = 0; st < kLowerStages; ++st) {
+      const int cnt = it / kLowerStages + (st < it % kLowerStages ? 1 : 0);
+      if (cnt > 0) drain_wait_cluster(bar(kF + st), uint32_t(cnt - 1) & 1u, status);
+    }
+  } else if (warp == 1 && issuer) {
+    mma_commit(bar(kD));
+    drain_wait_cluster(bar(kD), 0, status);
+  }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 256);
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -757,6 +793,26 @@ static int make_layout(int64_t m, int64_t n_kb, int64_t kc_blocks, int64_t w_row
   return H3_OK;
 }
 
+// Launch in clusters of `cluster` CTAs along x.
+template <typename... P, typename... A>
+static int launch_cluster(void (*kern)(P...), dim3 grid, int cluster, int threads, size_t smem, cudaStream_t st,
+                          A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) return H3_ERR_LAUNCH;
+  return cudaGetLastError() == cudaSuccess ? H3_OK : H3_ERR_LAUNCH;
+}
+
 template <typename K>
 static int allow_smem(K* kern, uint32_t bytes) {
   return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess
@@ -823,19 +879,9 @@ extern "C" int h3_gemm_adapters(const void* a, int64_t m, int64_t a_chunks, int6
     if ((rc = map_a(&tx, call, (unsigned)s.f.m_pad)) != H3_OK) return rc;
     if ((rc = make_map(&ta, lora_a, k, stacked, 1, lora_a_row_stride, stacked * lora_a_row_stride)) != H3_OK) return rc;
     if ((rc = allow_smem(few_lower_kernel, kFewLowerSmem)) != H3_OK) return rc;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(l.a_tiles * kSplitK));
-    cfg.blockDim = dim3(192);
-    cfg.dynamicSmemBytes = kFewLowerSmem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = kSplitK;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, few_lower_kernel, ta, tx, ad, s.f) != cudaSuccess) return H3_ERR_LAUNCH;
+    if ((rc = launch_cluster(few_lower_kernel, dim3((unsigned)(l.a_tiles * kSplitK)), kSplitK, 192, kFewLowerSmem, st, ta,
+                             tx, ad, s.f)) != H3_OK)
+      return rc;
     if ((rc = allow_smem(stream_kernel, kStreamSmem)) != H3_OK) return rc;
     if ((rc = launch_dependent(stream_kernel, dim3((unsigned)l.ctas), kStreamThreads, kStreamSmem, st, tw, tx, tb, ad,
                                s)) != H3_OK)
@@ -847,18 +893,22 @@ extern "C" int h3_gemm_adapters(const void* a, int64_t m, int64_t a_chunks, int6
   if ((rc = map_a(&tx, call)) != H3_OK) return rc;
   if ((rc = make_map(&ta, lora_a, k, stacked, 1, lora_a_row_stride, stacked * lora_a_row_stride, 64)) != H3_OK) return rc;
   int* chunks = reinterpret_cast<int*>(ws + l.low_bytes);
-  if ((rc = allow_smem(lower_kernel, kLowerSmem)) != H3_OK) return rc;
-  lower_kernel<<<(unsigned)((m + 127) / 128), 192, kLowerSmem, st>>>(tx, ta, ad, low, chunks, l.chunk_stride, (int)m,
-                                                                     p.n_kb, p.kc_blocks, status);
-  if (cudaGetLastError() != cudaSuccess) return H3_ERR_LAUNCH;
+  int sms = 0;
+  if ((rc = sm_count(sms)) != H3_OK) return rc;
+  // a cluster per tile of rows while their CTAs fit the SMs at once (see kQuarters)
+  const int64_t row_tiles = (m + 127) / 128;
+  const int cluster = row_tiles * kQuarters <= sms ? kQuarters : 1;
+  auto* lower = cluster > 1 ? lower_kernel<kQuarters> : lower_kernel<1>;
+  if ((rc = allow_smem(lower, kLowerSmem)) != H3_OK) return rc;
+  if ((rc = launch_cluster(lower, dim3((unsigned)(row_tiles * cluster)), cluster, 192, kLowerSmem, st, tx, ta, ad, low,
+                           chunks, l.chunk_stride, (int)m, p.n_kb, p.kc_blocks, status)) != H3_OK)
+    return rc;
   p.low = low;
   p.row_adapter = row_adapter;
   p.chunks = chunks;
   p.chunk_stride = l.chunk_stride;
   p.rank = (int)rank;
   p.n_adapters = (int)n_adapters;
-  int sms = 0;
-  if ((rc = sm_count(sms)) != H3_OK) return rc;
   constexpr uint32_t smem = smem_bytes(kNumBarsAdapters);
   if ((rc = allow_smem(adapter_gemm_kernel, smem)) != H3_OK) return rc;
   const int clusters = std::max(1, std::min(p.n_tiles, sms / 2));

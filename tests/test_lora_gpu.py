@@ -106,6 +106,16 @@ def test_a_row_does_not_depend_on_the_others(cuda_dev, m):
     assert torch.equal(O.linear_lora(x, w, a, b, scale, others)[0], y[0])
 
 
+def test_a_row_does_not_depend_on_the_calls_length(cuda_dev):
+    """Thousands of rows make T in one CTA a tile, hundreds in a cluster: the same bits."""
+    import h3attn as O
+    for k in (64, 136, 1088):
+        x, w, a, b, scale, rows = _case(cuda_dev, 5000, k, 136, 16, 9, 45, "scattered")
+        y = _check(O, (x, w, a, b, scale, rows))
+        for lo, hi in ((0, 100), (1000, 1700), (4935, 5000)):
+            assert torch.equal(O.linear_lora(x[lo:hi], w, a, b, scale, rows[lo:hi].contiguous()), y[lo:hi])
+
+
 @pytest.mark.parametrize("m", [30, 300])
 def test_adapters_that_no_row_uses_may_hold_anything(cuda_dev, m):
     """Whole groups of 64 stacked columns out of use, and A of any adapter that a row does not use itself."""
