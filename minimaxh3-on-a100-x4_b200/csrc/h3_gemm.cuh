@@ -177,7 +177,10 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmap_a, const CUten
           if (t == cid) pdl_wait();  // the chunk lists and low rows come from the kernel before
           const int* list = p.chunks + (long long)mb * p.chunk_stride;
           const int cnt = ok ? list[0] : 0;
+          int ids = 0;  // of 32 chunks, one a lane
           for (int i = 0; i < cnt; ++i, ++it) {
+            if ((i & 31) == 0) ids = i + lane < cnt ? list[1 + i + lane] : 0;
+            const int chunk = __shfl_sync(0xffffffffu, ids, i & 31);
             const int st = it % kStages;
             if (it >= kStages) {
               const int e = (it - kStages) / kRelEvery;
@@ -189,7 +192,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmap_a, const CUten
               mbar_arrive(bar(kLowFree + st));
               if (rank == 0) mbar_expect_tx(bar(kFull + st), 2 * kTileBytes);
               tma_load_3d_pair(sbase + st * kStageBytes + kTileBytes, &tmap_b, mapa_shared(bar(kFull + st), 0),
-                               64 * list[1 + i], w_row, 0);
+                               64 * chunk, w_row, 0);
             }
             __syncwarp();
           }
@@ -354,29 +357,37 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmap_a, const CUten
       const int row = mb * 256 + 128 * int(rank) + r_in;
       const int ad = row < p.m ? p.row_adapter[row] : -1;
       const int col0 = ad >= 0 && ad < p.n_adapters ? ad * p.rank : -1;  // first stacked column of the row's adapter
-      const __nv_bfloat16* src = p.low + (long long)row * p.rank;
-      for (int l = 0; l < cnt; ++l, ++it) {
-        const int st = it % kStages;
-        const int first = 64 * list[1 + l];  // the chunk's first stacked column
-        // the columns of this chunk that are the row's: pieces [at, at + pieces) of 8 columns, or none
-        const bool mine = col0 >= 0 && col0 < first + 64 && col0 + p.rank > first;
-        const int at = max(col0 - first, 0) / 8;
-        const uint4* from = reinterpret_cast<const uint4*>(src + max(first - col0, 0));
-        uint4 v[8];
+      const uint4* src = reinterpret_cast<const uint4*>(p.low + (long long)row * p.rank);
+      const int at = (max(col0, 0) & 63) / 8;  // the row's pieces of 8 columns in its (first) chunk: [at, at + pieces)
+      int held = col0 >= 0 ? col0 / 64 : -1;   // the chunk whose pieces v holds, loaded before they are needed
+      uint4 v[8];
+      auto hold = [&] {
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
           v[q] = make_uint4(0, 0, 0, 0);
-          if (mine && q >= at && q < at + pieces) v[q] = from[q - at];
+          if (held >= 0 && q >= at && q < at + pieces) v[q] = src[8 * (held - col0 / 64) + q - at];
         }
+      };
+      hold();
+      int ids = 0;  // of 32 chunks, one a lane
+      for (int l = 0; l < cnt; ++l, ++it) {
+        if ((l & 31) == 0) ids = l + lane < cnt ? list[1 + l + lane] : 0;
+        const int st = it % kStages;
+        const bool mine = __shfl_sync(0xffffffffu, ids, l & 31) == held;
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar(kLowFree + st), (free_par >> st) & 1u, ctx, kStatusTimeoutKV))))
           break;
         free_par ^= 1u << st;
         const uint32_t dst = sbase + st * kStageBytes + 128u * uint32_t(r_in);
 #pragma unroll
-        for (int q = 0; q < 8; ++q) st_shared_u4(dst + (uint32_t(q ^ (r_in & 7)) << 4), v[q]);
+        for (int q = 0; q < 8; ++q)
+          st_shared_u4(dst + (uint32_t(q ^ (r_in & 7)) << 4), mine ? v[q] : make_uint4(0, 0, 0, 0));
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive_remote_release(mapa_shared(bar(kLowFull + st), 0));
+        if (mine && 64 * (held + 1) < col0 + p.rank) {  // ranks above 64: the row's next chunk
+          ++held;
+          hold();
+        }
       }
     }
   }

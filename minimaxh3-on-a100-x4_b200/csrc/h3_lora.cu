@@ -19,9 +19,11 @@
 // 128-row tile, the chunks in use of the same rows of the stacked B against T (as above); they are dealt out
 // evenly to two CTAs per SM, and each CTA writes fp32 sums of the piece of a tile that it had. finish_kernel adds a
 // column's pieces in a fixed order, rounds and stores. Each launch is a programmatic dependent of the one before:
-// W streams while T is made, and a CTA leaves its piece with B for last. (B T by scalar code in finish_kernel took 15-25 us at 37 rows x 21504 columns.)
+// W streams while T is made, and a CTA leaves its piece with B for last. (B T by scalar code in finish_kernel took
+// 15-25 us at 37 rows x 21504 columns.)
 //
-// A row's value does not depend on the other rows of a call in either path (the paths differ in summation order).
+// Tile path: a row's bits do not depend on the other rows of the call or on its length. Row path: they do not depend on
+// the other rows' values, but where a column's pieces begin follows the chunks in use.
 #include <algorithm>
 
 #include "h3_gemm.cuh"
@@ -59,9 +61,12 @@ constexpr uint32_t kChunkBytes = 64u * 64u * 2u;
 constexpr uint32_t kLowerStage = kTileBytes + kPass * kChunkBytes;
 constexpr int kSumRow = 64 * kPass + 4;  // floats of a row of the cluster's sums (padded against bank conflicts)
 static_assert(128 * kSumRow * 4 <= kLowerStages * kLowerStage, "the sums reuse the ring");
+constexpr int kNoColumn = 1 << 30;
 struct LowerSmem {
   uint32_t own[kMaxChunks / 32], both[kMaxChunks / 32];  // chunks in use: these 128 rows, the block of 256
   uint16_t list[kMaxChunks];
+  int col0[128];     // first stacked column of each row's adapter, or kNoColumn
+  float scale[128];
   int count;
   uint64_t bars[2 * kLowerStages + 3];
   uint32_t tmem;
@@ -108,6 +113,10 @@ __global__ void __launch_bounds__(192, 1)
   for (int r = threadIdx.x; r < 256; r += 192) {
     const int row = (m0 & ~255) + r;
     const int a = adapter_of(ad, m, row);
+    if ((row & ~127) == m0) {
+      sh.col0[row - m0] = a < 0 ? kNoColumn : a * ad.rank;
+      sh.scale[row - m0] = a < 0 ? 0.f : ad.scale[a];
+    }
     if (a < 0) continue;
     const int last = (a * ad.rank + ad.rank - 1) / 64;
     for (int c = a * ad.rank / 64; c <= last; ++c) {
@@ -156,15 +165,15 @@ __global__ void __launch_bounds__(192, 1)
   float* sums = reinterpret_cast<float*>(smem);  // kCluster > 1: [128 rows][kSumRow] of this CTA's part, between passes
   int it = 0;                                    // ring items so far
   bool ok = run;
-  // Where a row's T goes: 8 stacked columns from `col` on, if they are its adapter's.
-  auto put = [&](int row, int col, const float (&v)[8]) {
-    const int a = adapter_of(ad, m, row);
-    if (a < 0 || col < a * ad.rank || col >= (a + 1) * ad.rank) return;
-    const float scale = ad.scale[a];
+  // Whether 8 stacked columns from `col` on are row r_in's adapter's, and where its T goes.
+  auto owns = [&](int r_in, int col) { return col >= sh.col0[r_in] && col < sh.col0[r_in] + ad.rank; };
+  auto put = [&](int r_in, int col, const float (&v)[8]) {
+    const float scale = sh.scale[r_in];
     uint32_t w[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(v[2 * e] * scale, v[2 * e + 1] * scale);
-    *reinterpret_cast<uint4*>(low + (long long)row * ad.rank + (col - a * ad.rank)) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(low + (long long)(m0 + r_in) * ad.rank + (col - sh.col0[r_in])) =
+        make_uint4(w[0], w[1], w[2], w[3]);
   };
 
   for (int ps = 0; ps < passes; ++ps) {
@@ -236,8 +245,8 @@ __global__ void __launch_bounds__(192, 1)
             const int col = 64 * sh.list[ps * kPass + i] + 16 * c;
             const float lo[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
             const float hi[8] = {v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15]};
-            put(m0 + r_in, col, lo);
-            put(m0 + r_in, col + 8, hi);
+            if (owns(r_in, col)) put(r_in, col, lo);
+            if (owns(r_in, col + 8)) put(r_in, col + 8, hi);
           }
         }
       tc_fence_before();
@@ -252,17 +261,24 @@ __global__ void __launch_bounds__(192, 1)
       constexpr int kRows = 128 / kCluster;
       for (int i = threadIdx.x; i < kRows * 8 * nc; i += 192) {
         const int r_in = kRows * rank + i / (8 * nc), piece = i % (8 * nc);
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = 0.f;
+        const int col = 64 * sh.list[ps * kPass + piece / 8] + 8 * (piece % 8);
+        if (!owns(r_in, col) || sh.abort != 0) continue;
+        float4 lo[kCluster], hi[kCluster];
         const uint32_t from = smem_u32(sums + r_in * kSumRow + 8 * piece);
 #pragma unroll
         for (int q = 0; q < kCluster; ++q) {
           const uint32_t at = mapa_shared(from, q);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] += ld_cluster_f32(at + 4u * e);
+          lo[q] = ld_cluster_f32x4(at);
+          hi[q] = ld_cluster_f32x4(at + 16u);
         }
-        if (sh.abort == 0) put(m0 + r_in, 64 * sh.list[ps * kPass + piece / 8] + 8 * (piece % 8), v);
+        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < kCluster; ++q) {
+          const float part_v[8] = {lo[q].x, lo[q].y, lo[q].z, lo[q].w, hi[q].x, hi[q].y, hi[q].z, hi[q].w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += part_v[e];
+        }
+        put(r_in, col, v);
       }
       cluster_sync_all();   // the sums have been read: the ring may be filled again
       fence_proxy_async();  // by the async proxy
@@ -667,32 +683,37 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
     const int a = adapter_of(ad, f.m, row);
     const int col0 = a >= 0 ? a * ad.rank : -1;
     const int pieces = min(ad.rank, 64) / 8;
-    const __nv_bfloat16* src = f.low + (long long)row * ad.rank;
+    const uint4* src = reinterpret_cast<const uint4*>(f.low + (long long)row * ad.rank);
+    const int at = (max(col0, 0) & 63) / 8;  // the row's pieces of 8 columns in its (first) chunk: [at, at + pieces)
     uint32_t free_par = 0;
     int it = 0;
     bool ok = true;
     pdl_wait();  // T comes from the kernel before
+    uint4 v[8];  // the pieces of the row's first chunk; with ranks up to 64 it has no other
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      v[e] = make_uint4(0, 0, 0, 0);
+      if (col0 >= 0 && e >= at && e < at + pieces) v[e] = src[e - at];
+    }
     for (long long g = g_end; ok && g > g_begin;) {
       const Piece q = piece(g);
       it += max(0, min(q.kb1, f.n_kb) - q.kb0);
       for (int kb = max(q.kb0, f.n_kb); kb < q.kb1; ++kb, ++it) {
         const int st = it % f.stages;
-        const int first = 64 * sh.list[kb - f.n_kb];  // the chunk's first stacked column
-        const bool mine = col0 >= 0 && col0 < first + 64 && col0 + ad.rank > first;
-        const int at = max(col0 - first, 0) / 8;
-        const uint4* from = reinterpret_cast<const uint4*>(src + max(first - col0, 0));
-        uint4 v[8];
+        const int beyond = sh.list[kb - f.n_kb] - max(col0, 0) / 64;  // the chunk, counted from the row's first
+        const bool mine = col0 >= 0 && beyond >= 0 && (beyond == 0 || 64 * beyond < ad.rank);
+        if (ad.rank > 64) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[e] = make_uint4(0, 0, 0, 0);
-          if (mine && e >= at && e < at + pieces) v[e] = from[e - at];
+          for (int e = 0; e < 8; ++e)
+            if (mine) v[e] = src[8 * beyond + e];
         }
         if (!(ok = __all_sync(0xffffffffu, mbar_wait(bar(kLE + st), (free_par >> st) & 1u, ctx, kStatusTimeoutKV)))) break;
         free_par ^= 1u << st;
         if (row < f.m_pad) {
           const uint32_t dst = sbase + st * stage_bytes + kTileBytes + 128u * uint32_t(row);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) st_shared_u4(dst + (uint32_t(e ^ (row & 7)) << 4), v[e]);
+          for (int e = 0; e < 8; ++e)
+            st_shared_u4(dst + (uint32_t(e ^ (row & 7)) << 4), mine ? v[e] : make_uint4(0, 0, 0, 0));
         }
         fence_proxy_async();
         __syncwarp();
@@ -830,8 +851,8 @@ extern "C" int64_t h3_gemm_adapters_workspace(int64_t m, int64_t a_chunks, int64
                                               int32_t epilogue, int64_t rank, int64_t n_adapters) {
   int rc;
   if (m < 1 || m > (1ll << 31) - 256 || a_chunks < 1 || a_chunks > 65535 || a_chunk_cols < 8 || n_out < 8 ||
-      a_chunk_cols > (1ll << 24) || a_chunk_cols * a_chunks > (1ll << 24) || n_out > (1ll << 30) || (epilogue != 0 && epilogue != 1) ||
-      2 * n_out * a_chunk_cols * a_chunks > (1ll << 41))
+      a_chunk_cols > (1ll << 24) || a_chunk_cols * a_chunks > (1ll << 24) || n_out > (1ll << 30) ||
+      (epilogue != 0 && epilogue != 1) || 2 * n_out * a_chunk_cols * a_chunks > (1ll << 41))
     return H3_ERR_SHAPE;
   if ((rc = check_adapters(rank, n_adapters)) != H3_OK) return rc;
   Layout l;

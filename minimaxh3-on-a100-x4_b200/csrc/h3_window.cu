@@ -227,7 +227,8 @@ __global__ void __launch_bounds__(Cfg<kTiles>::kThreads, Cfg<kTiles>::kCtasPerSm
       bool ok = true;
       Walk walk;
       int r = 0;
-      for (Item item = next_item<kTiles>(p, r, walk); ok && r < rounds_of<kTiles>(p); ++r, item = next_item<kTiles>(p, r, walk)) {
+      for (Item item = next_item<kTiles>(p, r, walk); ok && r < rounds_of<kTiles>(p);
+           ++r, item = next_item<kTiles>(p, r, walk)) {
         // Q is free once the last S of the item before is ready
         if (q_loads > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait(bar(C::kBarQFree), uint32_t(q_loads - 1) & 1u, ctx,
                                                                     kStatusTimeoutQ))))
@@ -553,7 +554,8 @@ __global__ void __launch_bounds__(Cfg<kTiles>::kThreads, Cfg<kTiles>::kCtasPerSm
             for (int e = 0; e < 4; ++e) d[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
           }
         }
-        if (valid && p.part_ml != nullptr) reinterpret_cast<float2*>(p.part_ml)[part] = make_float2(m_run, none ? 0.f : l_run);
+        if (valid && p.part_ml != nullptr)
+          reinterpret_cast<float2*>(p.part_ml)[part] = make_float2(m_run, none ? 0.f : l_run);
       }
     }
   }
@@ -805,7 +807,10 @@ struct Plan {
   int token;     // cluster size of token_kernel, or 0: window_kernel
 };
 
-// A single token with at most 4 query heads to a key head, and key heads enough that clusters of 8 CTAs reach most SMs:
+// A single token with at most 4 query heads to a key head, over few keys, or over a cache with key heads enough that clusters of
+// 8 CTAs fill the SMs three times (fewer do not keep enough loads in flight): 1000 keys of 8 / 28 / 56 heads 4.8 / 5.8 /
+// 8.2 us, by tiles 9.8 / 10.7 / 13.2; 2000: 6.6 / 10.2 / 14.8 and 10.1 / 13.0 / 19.5; 4000: 10.2 / 20.9 / 25.3 and
+// 11.2 / 19.8 / 28.1; 8000: 31 / 36 / 43.7 and 15.6 / 28.0 / 45.3; 16000: 61 / 67 / 81.8 and 20.8 / 44 / 80.1. It is
 // token_kernel, a CTA for 128 keys up to 8 of them. Else Q tiles of window_kernel: two per CTA (256 packed rows, one
 // CTA an SM) where the rows fill more than one, else one (two CTAs an SM); and splits only when the unsplit grid
 // leaves CTA slots empty: then as many as fill them, with at least two key tiles each.
@@ -838,7 +843,8 @@ static int make_plan(const Shape& s, int64_t splits_asked, Plan& pl) {
   pl.heads_turn = s.n_kv_heads * std::min(span, s.s_kv) * 512 <= (256ll << 20);
   const int64_t key_tiles = (std::min(span, s.s_kv) + kBlockN - 1) / kBlockN;
   pl.token = 0;
-  if (splits_asked == 0 && s.s_q == 1 && group <= 4 && s.n_kv_heads * kTokenMaxCluster >= sms) {
+  if (splits_asked == 0 && s.s_q == 1 && group <= 4 &&
+      (key_tiles <= 16 || (key_tiles <= 64 && s.n_kv_heads * kTokenMaxCluster >= 3 * sms))) {
     pl.token = (int)std::max<int64_t>(1, std::min<int64_t>(kTokenMaxCluster, key_tiles));
     pl.splits = pl.n_items = pl.ctas = 1;
     return H3_OK;

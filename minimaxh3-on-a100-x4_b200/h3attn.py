@@ -679,8 +679,8 @@ def linear_lora(a: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
       a, weight, out: as linear(); lora_a: [adapters * rank, k], lora_b: [weight rows, adapters * rank] bf16, adapter g at
       [g * rank, (g + 1) * rank) of both (stack_adapters lays them out); rank 8, 16, 32 or a multiple of 64 up to 256;
       scale: fp32 [adapters]; rows: int32 [m] (segment_rows makes it from token segments).
-    A row's bits do not depend on the other rows among calls of up to 64 rows, and among longer ones. B must be finite
-    where it is used: rows meet the adapters that share their group of 64 stacked columns with zero weights."""
+    In calls of more than 64 rows a row's bits do not depend on the other rows; up to 64 rows the order of its sums
+    follows which adapters the call uses. B must be finite where it is used: rows meet the adapters that share their group of 64 stacked columns with zero weights."""
     m, chunks, chunk_cols, chunk_stride, row_stride, n, ep, out = _linear_args(a, weight, out, epilogue)
     _cuda(lora_a, "lora_a")
     _cuda(lora_b, "lora_b")

@@ -95,6 +95,7 @@ def test_rows_without_an_adapter_are_the_projection(cuda_dev, m):
 
 @pytest.mark.parametrize("m", [50, 900])
 def test_a_row_does_not_depend_on_the_others(cuda_dev, m):
+    """Up to 64 rows: while the call uses the same adapters (each part here uses all of them)."""
     import h3attn as O
     x, w, a, b, scale, rows = _case(cuda_dev, m, 1088, 520, 32, 6, 40)
     y = O.linear_lora(x, w, a, b, scale, rows)

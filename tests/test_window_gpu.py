@@ -96,7 +96,7 @@ def test_more_blocks_than_ctas(cuda_dev, case, splits):
                                              splits=splits))
 
 
-@pytest.mark.parametrize("H,hk", [(20, 20), (40, 20), (57, 19), (80, 20), (100, 20)])
+@pytest.mark.parametrize("H,hk", [(1, 1), (20, 20), (40, 20), (57, 19), (80, 20), (100, 20), (60, 60), (240, 60)])
 @pytest.mark.parametrize("skv,left,right,sinks,q_start", [
     (1, 0, 0, 0, 0), (2, 0, 0, 1, 1), (63, None, 0, 0, 62), (64, 10, 0, 5, 63), (129, None, None, 0, 60),
     (1000, 300, 0, 100, 999), (1000, 300, 20, 700, 800), (5000, 4097, 0, 3, 4999), (777, 5, 5, 0, 5000),
