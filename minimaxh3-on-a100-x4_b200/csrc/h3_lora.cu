@@ -35,7 +35,9 @@ using namespace h3::gemm;
 
 constexpr int kMaxRank = 256;
 constexpr int kMaxChunks = 1024;  // n_adapters * rank <= 65536
-constexpr int kFewRows = 64;      // row path up to here
+// Row path up to here: 5376 -> 21504 with 24 adapters of rank 16, 64 rows 54 us, 65 rows by tiles 85; 7168 -> 5376 with 4,
+// 26 and 42. (Its accumulators and partial sums grow with the rows; the tiles cost the same up to 256.)
+constexpr int kFewRows = 64;
 
 struct Adapters {
   const int* row_adapter;
@@ -53,14 +55,20 @@ __device__ __forceinline__ int adapter_of(const Adapters& ad, int m, int r) {
 // cluster of kQuarters CTAs takes one part each (kCluster = 4) and the parts meet in distributed shared memory; with many, one
 // CTA takes them one after the other (kCluster = 1). Both give the same bits, so a row's T does not depend on the
 // call's length. One CTA per SM. 42000 rows of 7168: 99 us = 6.1 TB/s; whole calls of 1000 rows, 7168 -> 5376: 98 us with
-// one CTA per tile over all of k, 82 so; 65 rows of 5376 -> 21504: 86 and 77.
+// one CTA per tile over all of k, 82 so; 65 rows of 5376 -> 21504, 4 adapters of rank 32: 86 and 77.
 constexpr int kQuarters = 4;
-constexpr int kLowerStages = 6;
-constexpr int kPass = 2;  // chunks per pass over k: 16 KB of x and 2 x 8 KB of A per stage
 constexpr uint32_t kChunkBytes = 64u * 64u * 2u;
-constexpr uint32_t kLowerStage = kTileBytes + kPass * kChunkBytes;
-constexpr int kSumRow = 64 * kPass + 4;  // floats of a row of the cluster's sums (padded against bank conflicts)
-static_assert(128 * kSumRow * 4 <= kLowerStages * kLowerStage, "the sums reuse the ring");
+constexpr uint32_t kLowerRing = 192u * 1024u;
+constexpr int kLowerMaxStages = 6;
+template <int kCluster>
+struct Lower {
+  // Chunks per pass over k: tensor memory holds kQuarters parts of two, or a cluster's CTA its own part of four.
+  static constexpr int kPass = kCluster > 1 ? 4 : 2;
+  static constexpr uint32_t kStage = kTileBytes + kPass * kChunkBytes;
+  static constexpr int kStages = kLowerRing / kStage;
+  static constexpr int kSumRow = 64 * kPass + 4;  // floats of a row of the cluster's sums (padded against bank conflicts)
+  static_assert(kStages <= kLowerMaxStages && 128 * kSumRow * 4 <= kLowerRing, "the sums reuse the ring");
+};
 constexpr int kNoColumn = 1 << 30;
 struct LowerSmem {
   uint32_t own[kMaxChunks / 32], both[kMaxChunks / 32];  // chunks in use: these 128 rows, the block of 256
@@ -68,28 +76,32 @@ struct LowerSmem {
   int col0[128];     // first stacked column of each row's adapter, or kNoColumn
   float scale[128];
   int count;
-  uint64_t bars[2 * kLowerStages + 3];
+  uint64_t bars[2 * kLowerMaxStages + 3];
   uint32_t tmem;
   int abort;
 };
-constexpr uint32_t kLowerSmem = 1024 + kLowerStages * kLowerStage + sizeof(LowerSmem);
+constexpr uint32_t kLowerSmem = 1024 + kLowerRing + sizeof(LowerSmem);
 
 template <int kCluster>
 __global__ void __launch_bounds__(192, 1)
     lower_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_a,
                  const Adapters ad, __nv_bfloat16* low, int* chunks, int chunk_stride, int m, int n_kb, int kc_blocks,
                  int* status) {
+  constexpr int kPass = Lower<kCluster>::kPass, kLowerStages = Lower<kCluster>::kStages;
+  constexpr int kSumRow = Lower<kCluster>::kSumRow;
+  constexpr uint32_t kLowerStage = Lower<kCluster>::kStage;
   pdl_launch_dependents();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
-  LowerSmem& sh = *reinterpret_cast<LowerSmem*>(smem + kLowerStages * kLowerStage);
+  LowerSmem& sh = *reinterpret_cast<LowerSmem*>(smem + kLowerRing);
   enum { kF = 0, kE = kLowerStages, kAccF = 2 * kLowerStages, kAccE = kAccF + 1, kD = kAccE + 1 };
   auto bar = [&](int i) { return smem_u32(&sh.bars[i]); };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tile = blockIdx.x / kCluster, m0 = tile * 128;
   const int rank = kCluster > 1 ? int(cluster_ctarank()) : 0;
   const int q_begin = kCluster > 1 ? rank : 0, q_end = kCluster > 1 ? rank + 1 : kQuarters;  // this CTA's parts of k
+  auto acc = [&](int q, int i) { return 64u * uint32_t(kCluster > 1 ? i : kPass * q + i); };  // columns of part q, chunk i
   auto part = [&](int q) { return n_kb * q / kQuarters; };                                  // first k-block of part q
 
   for (int i = threadIdx.x; i < kMaxChunks / 32; i += 192) sh.own[i] = sh.both[i] = 0;
@@ -105,7 +117,7 @@ __global__ void __launch_bounds__(192, 1)
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(&sh.tmem), 512);  // part q, chunk i of the pass at 64 (kPass q + i)
+    tmem_alloc(smem_u32(&sh.tmem), 512);
     tmem_relinquish();
   }
   __syncthreads();
@@ -211,7 +223,7 @@ __global__ void __launch_bounds__(192, 1)
             const uint32_t x = sbase + st * kLowerStage;
             for (int i = 0; i < nc; ++i)
               for (int ks = 0; ks < 4; ++ks)
-                mma_ss(tmem + 64u * uint32_t(kPass * q + i), smem_desc_sw128(x + 32u * ks, 16, 1024),
+                mma_ss(tmem + acc(q, i), smem_desc_sw128(x + 32u * ks, 16, 1024),
                        smem_desc_sw128(x + kTileBytes + i * kChunkBytes + 32u * ks, 16, 1024), idesc,
                        kb > part(q) || ks > 0 ? 1u : 0u);
             mma_commit(bar(kE + st));
@@ -233,7 +245,7 @@ __global__ void __launch_bounds__(192, 1)
           for (int q = q_begin; q < q_end; ++q) {
             if (!ok || part(q) == part(q + 1)) continue;
             uint32_t r[16];
-            tmem_ld16_wait(tmem + lane_off + 64u * uint32_t(kPass * q + i) + 16u * c, r);
+            tmem_ld16_wait(tmem + lane_off + acc(q, i) + 16u * c, r);
 #pragma unroll
             for (int e = 0; e < 16; ++e) v[e] += __uint_as_float(r[e]);
           }

@@ -176,7 +176,7 @@ struct PackOut {
   const unsigned long long* rank_base;  // or one buffer per destination rank (peer memory)
   long long tensor_stride, row_offset;
   int heads_per_rank;
-  unsigned rank_magic;  // ceil(2^32 / heads_per_rank): h / heads_per_rank = h * magic >> 32 for h < 2^16, from 2 heads a rank
+  unsigned rank_magic;  // ceil(2^32 / heads_per_rank): h / heads_per_rank = h * magic >> 32, h < 2^16, from 2 a rank on
 };
 template <int kTensor>
 __device__ __forceinline__ __nv_bfloat16* pack_row(const PackOut& o, int h, long long tok) {
