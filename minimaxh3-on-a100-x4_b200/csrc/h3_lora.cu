@@ -42,7 +42,7 @@ constexpr int kFewRows = 64;
 struct Adapters {
   const int* row_adapter;
   const float* scale;
-  int n_adapters, rank, n_chunks;
+  int n_adapters, rank;
 };
 // the adapter of row r, or -1
 __device__ __forceinline__ int adapter_of(const Adapters& ad, int m, int r) {
@@ -897,7 +897,7 @@ extern "C" int h3_gemm_adapters(const void* a, int64_t m, int64_t a_chunks, int6
   if ((rc = make_layout(m, p.n_kb, p.kc_blocks, w_rows, rank, n_adapters, l)) != H3_OK) return rc;
   if (ws_bytes < l.bytes()) return H3_ERR_WORKSPACE;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const Adapters ad = {row_adapter, scale, (int)n_adapters, (int)rank, (int)((stacked + 63) / 64)};
+  const Adapters ad = {row_adapter, scale, (int)n_adapters, (int)rank};
   CUtensorMap tx, tw, ta, tb;
   if ((rc = map_w(&tw, call)) != H3_OK) return rc;
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
