@@ -354,9 +354,12 @@ class RopePositions:
     def __init__(self, pos: torch.Tensor, inv_freq: torch.Tensor, axis: torch.Tensor):
         self.pos, self.inv_freq, self.axis = pos, inv_freq, axis
 
-    def rows(self, lo: int, hi: int) -> "RopePositions":
-        """The positions of tokens [lo, hi); tokens past the last one (padding) sit at position 0."""
-        n = self.pos.shape[0]
+    def rows(self, lo: int, hi: int, tokens: int | None = None) -> "RopePositions":
+        """The positions of tokens [lo, hi) of a sequence of `tokens` (default: all that there are positions for);
+        tokens past its last one (padding) sit at position 0."""
+        n = self.pos.shape[0] if tokens is None else tokens
+        if not 0 <= n <= self.pos.shape[0]:
+            raise H3Error(f"positions of {self.pos.shape[0]} tokens, the sequence has {n}")
         pos = self.pos[min(lo, n):min(hi, n)]
         if pos.shape[0] < hi - lo:
             pos = torch.cat([pos, pos.new_zeros((hi - lo - pos.shape[0],) + tuple(pos.shape[1:]))])

@@ -734,7 +734,10 @@ def _sp_run_blocks(self, h, t_emb, mod_segments, rope_freqs, transformer_options
     h_loc = h_loc.contiguous()
     rope_loc = rope_loc.contiguous() if rope_loc is not None else None
     if _is_positions(rope_freqs):
-        rope_loc = rope_freqs.rows(lo, hi)
+        # as with a table: one row per token at least, rows behind the last token are not looked at
+        if rope_freqs.pos.shape[0] < S:
+            raise ValueError(f"rope_freqs holds positions of {rope_freqs.pos.shape[0]} tokens, the sequence has {S}")
+        rope_loc = rope_freqs.rows(lo, hi, S)
     segs_loc = _shard_segments(mod_segments, lo, hi)
     host_block = _host_block_timed if _TIMING else None
     _timeline = _Timeline(h_loc.is_cuda) if _TIMING else None
