@@ -211,13 +211,41 @@ def _attend(O, window, q, k, v, s_kv, layout, world=1):
 def set_adapters(linear, stacked) -> None:
     """Attach low-rank adapters to a projection of the host model (qkv_proj, out_proj, fc1 or fc2): stacked =
     (lora_a, lora_b, scale) of h3attn.stack_adapters, or None to take them off. They act in run_blocks calls that
-    name token segments in transformer_options["h3_adapter_segments"]."""
+    name token segments in transformer_options["h3_adapter_segments"]; such a call raises where they could not act.
+    A projection whose stack ends below a segment's adapter runs alone on that segment."""
     if stacked is None:
         if hasattr(linear, "h3_adapters"):
             del linear.h3_adapters
     else:
         lora_a, lora_b, scale = stacked
         linear.h3_adapters = (lora_a, lora_b, scale)
+
+
+def _adapted(*linears) -> bool:
+    return any(getattr(lin, "h3_adapters", None) is not None for lin in linears)
+
+
+def _check_adapters(model, segments, S) -> None:
+    """Raise where adapters would be dropped without a word: on a module that no patched forward routes through
+    _project, or a segment whose adapter no projection has (-1: none)."""
+    carrying = [m for m in model.modules() if _adapted(m)]
+    if not carrying:
+        return
+    routed = set()
+    for blk in model.blocks:
+        for part, forwards, names in (("attn", _ATTN_FORWARDS, ("qkv_proj", "out_proj")),
+                                      ("mlp", (_sp_mlp_forward,), ("fc1", "fc2"))):
+            part = getattr(blk, part, None)
+            if getattr(getattr(part, "forward", None), "__func__", None) in forwards:
+                routed.update(id(getattr(part, n, None)) for n in names)
+    if any(id(m) not in routed for m in carrying):
+        raise RuntimeError("sp_runtime: adapters are attached to a module that run_blocks does not apply them to "
+                           "(qkv_proj, out_proj of a block's attention and fc1, fc2 of its MLP take them)")
+    most = max(m.h3_adapters[2].shape[0] for m in carrying)
+    for a, b, adapter in segments:
+        if max(int(a), 0) < min(int(b), S) and not -1 <= int(adapter) < most:
+            raise ValueError(f"h3_adapter_segments: adapter {int(adapter)} of tokens [{a}, {b}), the projections have "
+                             f"{most} at most")
 
 
 def _project(O, lin, a, w, epilogue="none"):
@@ -278,7 +306,7 @@ def _gemm_weight(lin, x):
     elif w.dim() != 2 or w.device != x.device:
         why = "weight shape or device"
     if why is not None:
-        if _ADAPTER_ROWS is not None and getattr(lin, "h3_adapters", None) is not None:
+        if _ADAPTER_ROWS is not None and _adapted(lin):
             raise RuntimeError(f"sp_runtime: a projection with adapters cannot run on the library's GEMM ({why})")
         if x.is_cuda:
             _host_fallback("a projection", why)
@@ -291,6 +319,9 @@ def _sp_mlp_forward(self, x):
     SwiGLU fused into fc1's epilogue (cf. harness/sp_blockloop.py:167-170)."""
     w1, w2 = _gemm_weight(self.fc1, x), _gemm_weight(self.fc2, x)
     if not _SP_ACTIVE or w1 is None or w2 is None or x.dim() != 2:
+        if _ADAPTER_ROWS is not None and _adapted(self.fc1, self.fc2):
+            raise RuntimeError("sp_runtime: an MLP with adapters cannot run on the host module's ops (an input of "
+                               f"shape {tuple(x.shape)}, or a projection that the library's GEMM does not take)")
         return _orig_mlp_forward(self, x)
     O = ops()
     return _project(O, self.fc2, _project(O, self.fc1, x, w1, "swiglu"), w2)
@@ -630,6 +661,10 @@ def _sp_attn_forward_ce(self, x, rope_freqs=None, transformer_options={}):
         return self.out_proj(O.head_to_seq_unpack(o_heads))
 
 
+_ATTN_FORWARDS = (_sp_attn_forward, _sp_attn_forward_overlap, _sp_attn_forward_heads, _sp_attn_forward_peer,
+                  _sp_attn_forward_ce)
+
+
 def _shard_segments(segs, lo, hi):
     out = []
     for a, b, row in segs:
@@ -746,6 +781,7 @@ def _sp_run_blocks(self, h, t_emb, mod_segments, rope_freqs, transformer_options
     try:
         adapter_segs = (transformer_options or {}).get("h3_adapter_segments")
         if adapter_segs:
+            _check_adapters(self, adapter_segs, S)
             _ADAPTER_ROWS = ops().segment_rows(_shard_segments(adapter_segs, lo, hi), h_loc.shape[0], h_loc.device)
         for blk in self.blocks:
             if _fusable(blk, h_loc):

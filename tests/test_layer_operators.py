@@ -86,3 +86,67 @@ def test_rows_of_positions():
     assert rp.rows(4, 6, 4).pos[:, 0].tolist() == [0, 0]
     with pytest.raises(O.H3Error):
         rp.rows(0, 6, 6)
+
+
+def _adapters(lin, count):
+    import h3attn as O
+    n, k = lin.weight.shape
+    g = torch.Generator().manual_seed(n + k)
+    pairs = [(torch.randn(8, k, generator=g) * k ** -0.5, torch.randn(n, 8, generator=g)) for _ in range(count)]
+    return O.stack_adapters(pairs, [1.0] * count)
+
+
+def _run_adapted(M, model, S, segments):
+    import sp_runtime
+    h = torch.randn(S, 64, generator=torch.Generator().manual_seed(4)).bfloat16()
+    with torch.no_grad():
+        return sp_runtime._sp_run_blocks(model, h, torch.ones(1, 16).bfloat16(), [(0, S, 0)], None,
+                                         {"h3_adapter_segments": segments})
+
+
+@pytest.mark.parametrize("where", ["adaln", "unpatched mlp", "fc2 with a bias", "3-D input"])
+def test_adapters_that_could_not_act_are_an_error(monkeypatch, where):
+    import sp_runtime
+    S = 6
+    M, model, _ = _one_block(S, monkeypatch, S)
+    blk = model.blocks[0]
+    lin = blk.adaln_proj.lin if where == "adaln" else blk.mlp.fc1
+    sp_runtime.set_adapters(lin, _adapters(lin, 2))
+    if where == "fc2 with a bias":  # fc1's adapters must not go with fc2's fall back to the host's MLP
+        blk.mlp.fc2.bias = torch.nn.Parameter(torch.zeros(64, dtype=torch.bfloat16))
+    elif where == "3-D input":
+        blk.mlp.register_forward_pre_hook(lambda m, x: (x[0][None],))
+    elif where == "unpatched mlp":
+        monkeypatch.setattr(M, "MLP", torch.nn.Identity)  # not the class of the block's MLP
+    sp_runtime.install(M)
+    try:
+        _run_adapted(M, model, S, [])  # no segments: the bare model
+        with pytest.raises(RuntimeError, match="adapters"):
+            _run_adapted(M, model, S, [(0, S, 0)])
+        assert sp_runtime._ADAPTER_ROWS is None and not sp_runtime._SP_ACTIVE
+    finally:
+        sp_runtime.uninstall()
+
+
+def test_adapter_numbers_of_segments(monkeypatch):
+    """A number that no projection's stack reaches is an error; one that some stack has acts there and there alone."""
+    import sp_runtime
+    S = 6
+    M, model, _ = _one_block(S, monkeypatch, S)
+    blk = model.blocks[0]
+    blk.adaln_proj.lin.bias.data.fill_(1.0)
+    sp_runtime.install(M)
+    try:
+        bare = _run_adapted(M, model, S, [(0, S, 5)])  # nothing attached: nothing to reach
+        sp_runtime.set_adapters(blk.attn.qkv_proj, _adapters(blk.attn.qkv_proj, 3))
+        for bad in ([(0, 2, 0), (2, S, 3)], [(0, S, -2)]):
+            with pytest.raises(ValueError, match="h3_adapter_segments"):
+                _run_adapted(M, model, S, bad)
+        assert torch.equal(_run_adapted(M, model, S, [(0, S, -1), (S, S + 4, 9), (3, 3, 9)]), bare)
+        last = _run_adapted(M, model, S, [(0, S, 2)])
+        assert not torch.equal(last, bare)
+        sp_runtime.set_adapters(blk.mlp.fc2, _adapters(blk.mlp.fc2, 2))
+        assert torch.equal(_run_adapted(M, model, S, [(0, S, 2)]), last)
+        assert not torch.equal(_run_adapted(M, model, S, [(0, S, 1)]), last)
+    finally:
+        sp_runtime.uninstall()
