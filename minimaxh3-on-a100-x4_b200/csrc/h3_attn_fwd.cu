@@ -411,7 +411,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = __all_sync(0xffffffffu, mbar_wait(bar(kBarSFull + t), uint32_t(j) & 1u, ctx, kStatusTimeoutS));
       if (!ok) break;
       // S_1(j) ready: every MMA reading K_j and V_(j-1) has retired; hand their stages back
-      if (t == 1 && quad == 0 && lane == 0) mbar_arrive(bar(kBarRel + j % kRel));
+      if (t == 1 && quad == 0) {
+        if (lane == 0) mbar_arrive(bar(kBarRel + j % kRel));
+        __syncwarp();
+      }
       prof_mark<kProf>(p, rec, t, j, 1);
       tc_fence_after();
       // S in two 64-column halves: the second half's load is in flight while the first half's
@@ -474,6 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             l_b = f2_fma(l_b, f2_pack(f, f), f2_pack(0.f, 0.f));
             m_run = m_new;
           }
+          __syncwarp();
 #pragma unroll 1
           for (int c16 = 0; c16 < 8; ++c16) {
             uint32_t o[16];
@@ -561,6 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) d4[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
         }
+        __syncwarp();  // the next load of O takes the whole warp
       }
     }
     if (peer) {

@@ -302,6 +302,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmap_a, const CUten
                 *reinterpret_cast<uint4*>(dst + 32 * c32 + 8 * q) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2],
                                                                                 w[4 * q + 3]);
           }
+          __syncwarp();  // the next load of the accumulators takes the whole warp
         }
       } else {
         // out = bf16(bf16(silu(g)) * u), g and u the bf16-rounded gate / up projections
@@ -331,6 +332,7 @@ __device__ __forceinline__ void gemm_body(const CUtensorMap& tmap_a, const CUten
               *reinterpret_cast<uint4*>(dst + 32 * c32 + 8 * q) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2],
                                                                               w[4 * q + 3]);
           }
+          __syncwarp();
         }
       }
       tc_fence_before();

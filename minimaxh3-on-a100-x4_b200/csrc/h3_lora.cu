@@ -259,6 +259,7 @@ __global__ void __launch_bounds__(192, 1)
             const float hi[8] = {v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15]};
             if (owns(r_in, col)) put(r_in, col, lo);
             if (owns(r_in, col + 8)) put(r_in, col + 8, hi);
+            __syncwarp();  // the next load of the accumulators takes the whole warp
           }
         }
       tc_fence_before();

@@ -396,9 +396,12 @@ __global__ void __launch_bounds__(Cfg<kTiles>::kThreads, Cfg<kTiles>::kCtasPerSm
       for (int j = 0; ok && j < item.n_kv; ++j, ++jg) {
         ok = __all_sync(0xffffffffu, mbar_wait(bar(C::kBarS + t), uint32_t(jg) & 1u, ctx, kStatusTimeoutS));
         if (!ok) break;
-        if (t == kTiles - 1 && quad == 0 && lane == 0) {
-          mbar_arrive(bar(C::kBarRel + jg % C::kRel));
-          if (j + 1 == item.n_kv) mbar_arrive(bar(C::kBarQFree));  // every S of this item is done: Q may be replaced
+        if (t == kTiles - 1 && quad == 0) {
+          if (lane == 0) {
+            mbar_arrive(bar(C::kBarRel + jg % C::kRel));
+            if (j + 1 == item.n_kv) mbar_arrive(bar(C::kBarQFree));  // every S of this item is done: Q may be replaced
+          }
+          __syncwarp();
         }
         tc_fence_after();
         const int key = walk.base(item.j_lo + j);
@@ -469,6 +472,7 @@ __global__ void __launch_bounds__(Cfg<kTiles>::kThreads, Cfg<kTiles>::kCtasPerSm
               l_b = f2_fma(l_b, f2_pack(f, f), f2_pack(0.f, 0.f));
               m_run = m_new;
             }
+            __syncwarp();
 #pragma unroll 1
             for (int c16 = 0; c16 < 8; ++c16) {
               uint32_t o[16];
@@ -536,15 +540,14 @@ __global__ void __launch_bounds__(Cfg<kTiles>::kThreads, Cfg<kTiles>::kCtasPerSm
         for (int c4 = 0; c4 < 4; ++c4) {
           uint32_t o[32];
           tmem_ld32_wait(tO + c4 * 32, o);
-          if (!valid) continue;
-          if (p.part_o != nullptr) {
+          if (valid && p.part_o != nullptr) {
             float4* d = reinterpret_cast<float4*>(p.part_o + part * 128 + c4 * 32);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
               d[e] = none ? make_float4(0.f, 0.f, 0.f, 0.f)
                           : make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
                                         __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
-          } else {
+          } else if (valid) {
             uint32_t w[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e)
@@ -553,6 +556,7 @@ __global__ void __launch_bounds__(Cfg<kTiles>::kThreads, Cfg<kTiles>::kCtasPerSm
 #pragma unroll
             for (int e = 0; e < 4; ++e) d[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
           }
+          __syncwarp();  // the next load of O takes the whole warp
         }
         if (valid && p.part_ml != nullptr)
           reinterpret_cast<float2*>(p.part_ml)[part] = make_float2(m_run, none ? 0.f : l_run);

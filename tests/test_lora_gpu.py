@@ -232,3 +232,20 @@ def test_refusals(cuda_dev):
         O.linear_lora(x, w, a, b, scale, rows, epilogue="gelu")
     with pytest.raises(O.H3Error):
         O.linear_lora(x, w, a, b, scale, rows, epilogue="swiglu")  # 32 columns, not a multiple of 128
+
+
+@pytest.mark.parametrize("m", [1, 3, 7, 13, 21, 35, 51, 63])
+@pytest.mark.parametrize("rank,na", [(8, 3), (16, 9), (64, 2)])
+def test_odd_row_counts(cuda_dev, m, rank, na):
+    """Odd counts end the loop over a cluster's sums in the middle of a warp, in front of the cluster barrier."""
+    import h3attn as O
+    for k, n in ((8, 264), (1096, 136)):
+        _check(O, _case(cuda_dev, m, k, n, rank, na, 130 + m))
+
+
+@pytest.mark.parametrize("m", [65, 131, 259, 601])
+def test_scattered_rows_of_few_columns(cuda_dev, m):
+    """Neighbouring rows of other adapters part the lanes of a warp at every piece of T, with clusters and without."""
+    import h3attn as O
+    for rank, na in ((8, 40), (16, 24), (128, 5)):
+        _check(O, _case(cuda_dev, m, 328, 136, rank, na, 140 + m))

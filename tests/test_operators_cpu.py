@@ -217,3 +217,14 @@ def test_rank_of_a_head_by_multiplication():
         assert magic < 2 ** 32
         for h in {0, 1, per - 1, per, min(per + 1, 65535), min(2 * per - 1, 65535), 65534, 65535 - 65535 % per, 65535}:
             assert h * magic >> 32 == h // per
+
+
+def test_whole_warps_at_cluster_barriers_and_tensor_memory():
+    """Cluster barriers and the release of tensor memory take whole warps (.aligned): their wrappers bring the warp
+    together themselves, whatever the code before them left."""
+    import re
+    here = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = open(os.path.join(here, "minimaxh3-on-a100-x4_b200", "csrc", "h3_ptx.cuh")).read()
+    for name in ("cluster_sync_all", "tmem_dealloc", "tmem_dealloc_pair"):
+        body = re.search(r"void %s\([^)]*\) \{\n(.*?)\n\}" % name, src, re.S).group(1)
+        assert body.lstrip().startswith("__syncwarp();"), name
