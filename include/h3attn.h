@@ -242,11 +242,13 @@ int h3_gemm_bf16(const void* a, int64_t m, int64_t a_chunks, int64_t a_chunk_col
  * adapter g from g * rank), bf16, row strides multiples of 8; rank 8, 16, 32 or a multiple of 64 up to 256 (a smaller
  * one is padded with zeros), n_adapters * rank <= 65536; scale fp32 [n_adapters], row_adapter int32 [m]. fp32
  * accumulation; scale * A_g a[t] is rounded to bf16. The bits of an output row do not depend on the other rows nor
- * on m in calls of m > 64; up to 64 rows the order of its sums follows which adapters the call uses. lora_b must be finite in the groups of 64 stacked columns that a row of the call
- * uses: other rows of the same 256 (of the call, up to 64 rows) meet them with zero weights. Elsewhere the stacks may
- * hold anything.
+ * on m in calls of m > 64, nor in any call whose epilogue carries H3_GEMM_ROW_INDEPENDENT (epilogue | flag; a row without
+ * an adapter then has the bits of h3_gemm_bf16); else, up to 64 rows, the order of its sums follows which adapters the
+ * call uses. lora_b must be finite in the groups of 64 stacked columns that a row of the call uses: other rows of the
+ * same 256 (of the call, up to 64 rows) meet them with zero weights. Elsewhere the stacks may hold anything.
  * h3_gemm_adapters_workspace returns the bytes of 16-byte aligned workspace that the call needs (or an error); it may
  * be reused once the call's work on the stream is done. */
+#define H3_GEMM_ROW_INDEPENDENT 0x100
 int64_t h3_gemm_adapters_workspace(int64_t m, int64_t a_chunks, int64_t a_chunk_cols, int64_t n_out, int32_t epilogue,
                                    int64_t rank, int64_t n_adapters);
 int h3_gemm_adapters(const void* a, int64_t m, int64_t a_chunks, int64_t a_chunk_cols, int64_t a_chunk_stride,

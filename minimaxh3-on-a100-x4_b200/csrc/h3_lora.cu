@@ -23,7 +23,8 @@
 // 15-25 us at 37 rows x 21504 columns.)
 //
 // Tile path: a row's bits do not depend on the other rows of the call or on its length. Row path: they do not depend on
-// the other rows' values, but where a column's pieces begin follows the chunks in use.
+// the other rows' values, but where a column's pieces begin follows the chunks in use. A caller that needs the first
+// whatever the length (shards of one sequence) asks for tiles with H3_GEMM_ROW_INDEPENDENT.
 #include <algorithm>
 
 #include "h3_gemm.cuh"
@@ -798,10 +799,10 @@ static int check_adapters(int64_t rank, int64_t n_adapters) {
 }
 
 static int make_layout(int64_t m, int64_t n_kb, int64_t kc_blocks, int64_t w_rows, int64_t rank, int64_t n_adapters,
-                       Layout& l) {
+                       bool tiles, Layout& l) {
   l = {};
   const int64_t stacked = rank * n_adapters;
-  l.few = m <= kFewRows;
+  l.few = !tiles && m <= kFewRows;
   l.low_bytes = (m * rank * 2 + 255) / 256 * 256;
   if (!l.few) {
     l.chunk_stride = 1 + (int)((stacked + 63) / 64);
@@ -863,6 +864,8 @@ using namespace h3::lora;
 extern "C" int64_t h3_gemm_adapters_workspace(int64_t m, int64_t a_chunks, int64_t a_chunk_cols, int64_t n_out,
                                               int32_t epilogue, int64_t rank, int64_t n_adapters) {
   int rc;
+  const bool tiles = (epilogue & H3_GEMM_ROW_INDEPENDENT) != 0;
+  epilogue &= ~H3_GEMM_ROW_INDEPENDENT;
   if (m < 1 || m > (1ll << 31) - 256 || a_chunks < 1 || a_chunks > 65535 || a_chunk_cols < 8 || n_out < 8 ||
       a_chunk_cols > (1ll << 24) || a_chunk_cols * a_chunks > (1ll << 24) || n_out > (1ll << 30) ||
       (epilogue != 0 && epilogue != 1) || 2 * n_out * a_chunk_cols * a_chunks > (1ll << 41))
@@ -870,7 +873,8 @@ extern "C" int64_t h3_gemm_adapters_workspace(int64_t m, int64_t a_chunks, int64
   if ((rc = check_adapters(rank, n_adapters)) != H3_OK) return rc;
   Layout l;
   const int64_t kc = (a_chunk_cols + 63) / 64;
-  if ((rc = make_layout(m, kc * a_chunks, kc, epilogue == 1 ? 2 * n_out : n_out, rank, n_adapters, l)) != H3_OK) return rc;
+  if ((rc = make_layout(m, kc * a_chunks, kc, epilogue == 1 ? 2 * n_out : n_out, rank, n_adapters, tiles, l)) != H3_OK)
+    return rc;
   return l.bytes();
 }
 
@@ -880,6 +884,8 @@ extern "C" int h3_gemm_adapters(const void* a, int64_t m, int64_t a_chunks, int6
                                 const void* lora_b, int64_t lora_b_row_stride, int64_t rank, int64_t n_adapters,
                                 const float* scale, const int32_t* row_adapter, void* c, int64_t c_row_stride,
                                 int32_t epilogue, void* workspace, int64_t ws_bytes, int32_t* status, void* stream) {
+  const bool tiles = (epilogue & H3_GEMM_ROW_INDEPENDENT) != 0;
+  epilogue &= ~H3_GEMM_ROW_INDEPENDENT;
   const Call call = {a, m, a_chunks, a_chunk_cols, a_chunk_stride, a_row_stride, w, n_out, w_row_stride, c,
                      c_row_stride, epilogue, status};
   int rc;
@@ -895,7 +901,7 @@ extern "C" int h3_gemm_adapters(const void* a, int64_t m, int64_t a_chunks, int6
     return H3_ERR_STRIDE;
   Params p = call_params(call);
   Layout l;
-  if ((rc = make_layout(m, p.n_kb, p.kc_blocks, w_rows, rank, n_adapters, l)) != H3_OK) return rc;
+  if ((rc = make_layout(m, p.n_kb, p.kc_blocks, w_rows, rank, n_adapters, tiles, l)) != H3_OK) return rc;
   if (ws_bytes < l.bytes()) return H3_ERR_WORKSPACE;
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const Adapters ad = {row_adapter, scale, (int)n_adapters, (int)rank};

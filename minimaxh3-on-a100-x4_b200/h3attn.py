@@ -637,6 +637,7 @@ def linear(a: torch.Tensor, weight: torch.Tensor, out: torch.Tensor | None = Non
 
 # ----------------------------------------------------------------------------- adapters beside a projection
 _RANKS = (8, 16, 32, 64, 128, 192, 256)
+_ROW_INDEPENDENT = 0x100  # H3_GEMM_ROW_INDEPENDENT
 
 
 def stack_adapters(pairs, scales, device=None):
@@ -676,14 +677,16 @@ def _adapters_workspace(dev_index: int, *shape) -> int:
 
 def linear_lora(a: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
                 scale: torch.Tensor, rows: torch.Tensor, out: torch.Tensor | None = None,
-                epilogue: str = "none") -> torch.Tensor:
+                epilogue: str = "none", row_independent: bool = False) -> torch.Tensor:
     """linear() with a low-rank adapter per row: a @ weight.T + scale[g] * (a @ A_g.T) @ B_g.T with g = rows[row]
     (outside [0, adapters): the projection alone), rounded once; epilogue "swiglu" as linear().
       a, weight, out: as linear(); lora_a: [adapters * rank, k], lora_b: [weight rows, adapters * rank] bf16, adapter g at
       [g * rank, (g + 1) * rank) of both (stack_adapters lays them out); rank 8, 16, 32 or a multiple of 64 up to 256;
       scale: fp32 [adapters]; rows: int32 [m] (segment_rows makes it from token segments).
-    In calls of more than 64 rows a row's bits do not depend on the other rows; up to 64 rows the order of its sums
-    follows which adapters the call uses. B must be finite where it is used: rows meet the adapters that share their group of 64 stacked columns with zero weights."""
+    In calls of more than 64 rows a row's bits do not depend on the other rows, and a row without an adapter has
+    linear()'s bits; up to 64 rows the order of its sums follows which adapters the call uses, unless row_independent is
+    set (slower: for shards of one sequence that must agree bit for bit whatever their lengths). B must be finite where
+    it is used: rows meet the adapters that share their group of 64 stacked columns with zero weights."""
     m, chunks, chunk_cols, chunk_stride, row_stride, n, ep, out = _linear_args(a, weight, out, epilogue)
     _cuda(lora_a, "lora_a")
     _cuda(lora_b, "lora_b")
@@ -701,6 +704,8 @@ def linear_lora(a: torch.Tensor, weight: torch.Tensor, lora_a: torch.Tensor, lor
     if rows.shape != (m,) or not rows.is_contiguous():
         raise H3Error(f"rows must be a contiguous int32 [{m}]")
     rank = lora_a.shape[0] // n_adapters
+    if row_independent:
+        ep |= _ROW_INDEPENDENT
     with _on(dev):
         ws_bytes = _adapters_workspace(dev, m, chunks, chunk_cols, n, ep, rank, n_adapters)
         ws = a.new_empty(((ws_bytes + 1) // 2,))

@@ -249,11 +249,12 @@ def _check_adapters(model, segments, S) -> None:
 
 
 def _project(O, lin, a, w, epilogue="none"):
-    """a @ w.T on the library's GEMM, with the projection's adapters where this call has adapter rows."""
+    """a @ w.T on the library's GEMM, with the projection's adapters where this call has adapter rows (by the kernels
+    whose rows do not depend on the shard's length)."""
     ad = getattr(lin, "h3_adapters", None)
     if ad is None or _ADAPTER_ROWS is None:
         return O.linear(a, w) if epilogue == "none" else O.linear(a, w, epilogue=epilogue)
-    return O.linear_lora(a, w, *ad, _ADAPTER_ROWS, epilogue=epilogue)
+    return O.linear_lora(a, w, *ad, _ADAPTER_ROWS, epilogue=epilogue, row_independent=True)
 
 
 def _norm_inputs(self, x, rope_freqs):

@@ -121,7 +121,7 @@ def window_attention(q, k, v, left, right, sinks=0, causal=False, q_start=None, 
     return o
 
 
-def linear_lora(a, weight, lora_a, lora_b, scale, rows, out=None, epilogue="none"):
+def linear_lora(a, weight, lora_a, lora_b, scale, rows, out=None, epilogue="none", row_independent=False):
     if a.dim() == 3:
         a = a.transpose(0, 1).reshape(a.shape[1], -1)
     na = scale.shape[0]

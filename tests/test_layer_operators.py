@@ -150,3 +150,22 @@ def test_adapter_numbers_of_segments(monkeypatch):
         assert not torch.equal(_run_adapted(M, model, S, [(0, S, 1)]), last)
     finally:
         sp_runtime.uninstall()
+
+
+def test_projections_with_adapters_do_not_depend_on_the_shard(monkeypatch):
+    """The runtime asks for kernels whose rows have the same bits in a shard of any length."""
+    import sp_runtime
+    S = 6
+    M, model, _ = _one_block(S, monkeypatch, S)
+    blk, asked = model.blocks[0], []
+    for lin in (blk.attn.qkv_proj, blk.attn.out_proj, blk.mlp.fc1, blk.mlp.fc2):
+        sp_runtime.set_adapters(lin, _adapters(lin, 1))
+    plain = sp_runtime.ops().linear_lora
+    monkeypatch.setattr(sp_runtime.ops(), "linear_lora",
+                        lambda *a, **k: asked.append(k.get("row_independent")) or plain(*a, **k))
+    sp_runtime.install(M)
+    try:
+        _run_adapted(M, model, S, [(0, 3, 0)])
+    finally:
+        sp_runtime.uninstall()
+    assert asked == [True] * 4

@@ -27,3 +27,14 @@ def test_across_gpus(world, overlap, tmp_path):
     for k in one:
         # token pieces start the window's key walk at other rows: equal values, not equal bits
         assert T.near(many[k], one[k]) if overlap == "1" else torch.equal(many[k], one[k])
+
+
+@pytest.mark.parametrize("world", [2, 4])
+def test_short_shards_with_adapters_across_gpus(world, tmp_path):
+    """Shards of 64 rows and fewer, where one GPU has more: the same bits."""
+    if torch.cuda.device_count() < world:
+        pytest.skip(f"needs {world} GPUs")
+    for S in (101, 203):
+        one, many = T.run(1, S, tmp_path, on_gpu=True), T.run(world, S, tmp_path, on_gpu=True)
+        for k in ("dense", "out"):
+            assert torch.equal(many[k], one[k]), (S, k)

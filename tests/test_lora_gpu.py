@@ -249,3 +249,26 @@ def test_scattered_rows_of_few_columns(cuda_dev, m):
     import h3attn as O
     for rank, na in ((8, 40), (16, 24), (128, 5)):
         _check(O, _case(cuda_dev, m, 328, 136, rank, na, 140 + m))
+
+
+@pytest.mark.parametrize("rank,na", [(8, 5), (16, 24), (128, 3)])
+def test_row_independent_calls_of_any_length(cuda_dev, rank, na):
+    """Shards of a sequence have the bits of the whole, however short: 1000 rows in pieces of 1 to 64, both epilogues,
+    head-major input; rows without an adapter have the projection's own."""
+    import h3attn as O
+    x, w, a, b, scale, rows = _case(cuda_dev, 1000, 640, 512, rank, na, 150 + rank)
+    heads = x.view(1000, 5, 128).transpose(0, 1).contiguous()
+    for ep in ("none", "swiglu"):
+        whole, base = O.linear_lora(x, w, a, b, scale, rows, epilogue=ep), O.linear(x, w, epilogue=ep)
+        bare = rows < 0
+        for lo, n in ((0, 1), (5, 50), (500, 64), (936, 64), (983, 17)):
+            r = rows[lo:lo + n].contiguous()
+            y = O.linear_lora(x[lo:lo + n], w, a, b, scale, r, epilogue=ep, row_independent=True)
+            assert torch.equal(y, whole[lo:lo + n]), (ep, lo, n)
+            at = bare[lo:lo + n]
+            assert torch.equal(y[at], base[lo:lo + n][at])
+            part = heads[:, lo:lo + n].contiguous()
+            assert torch.equal(O.linear_lora(part, w, a, b, scale, r, epilogue=ep, row_independent=True), y)
+        assert torch.equal(O.linear_lora(x, w, a, b, scale, rows, epilogue=ep, row_independent=True), whole)
+    O.check_status()
+    _check(O, (x[:33], w, a, b, scale, rows[:33].contiguous()), row_independent=True)

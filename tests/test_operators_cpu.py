@@ -228,3 +228,20 @@ def test_whole_warps_at_cluster_barriers_and_tensor_memory():
     for name in ("cluster_sync_all", "tmem_dealloc", "tmem_dealloc_pair"):
         body = re.search(r"void %s\([^)]*\) \{\n(.*?)\n\}" % name, src, re.S).group(1)
         assert body.lstrip().startswith("__syncwarp();"), name
+
+
+def test_row_independent_adapters_take_the_tiles(L):
+    """The flag asks for the launch whose rows do not depend on the call's length: its workspace grows with the rows
+    and the chunk lists alone, also below 65 rows, and needs no device to size."""
+    flag = 0x100
+    tiles = lambda m: (m * 16 * 2 + 255) // 256 * 256 + (m + 255) // 256 * (1 + 1) * 4  # noqa: E731
+    for m in (1, 40, 64, 65, 300):
+        assert L.h3_gemm_adapters_workspace(m, 1, 512, 256, flag, 16, 4) == tiles(m)
+        assert L.h3_gemm_adapters_workspace(m, 1, 512, 256, flag | 1, 16, 4) == tiles(m)
+    assert L.h3_gemm_adapters_workspace(300, 1, 512, 256, 0, 16, 4) == tiles(300)
+    assert L.h3_gemm_adapters_workspace(300, 1, 512, 256, flag | 2, 16, 4) == -3
+    assert L.h3_gemm_adapters_workspace(300, 1, 512, 256, 2 * flag, 16, 4) == -3
+    p, st = ctypes.c_void_p(0x1000), ctypes.c_void_p(0x2000)
+    ok = [p, 20, 1, 512, 0, 512, p, 256, 512, p, 512, p, 64, 16, 4, p, p, p, 256, flag, p, 0, st, None]
+    assert L.h3_gemm_adapters(*ok) == -12
+    assert L.h3_gemm_adapters(*(ok[:19] + [flag | 2] + ok[20:])) == -3
