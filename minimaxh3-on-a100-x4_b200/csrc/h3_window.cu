@@ -785,7 +785,7 @@ __global__ void __launch_bounds__(32 * kTokenWarps) token_kernel(const Params p,
 }
 
 // ---------------------------------------------------------------- host
-constexpr int64_t kMaxPos = 1ll << 29;  // positions, window sides and lengths stay inside int32 sums
+constexpr int64_t kMaxPos = 1ll << 29;  // lengths and |q_start|: positions lie in [-2^29, 2^30)
 constexpr int kMaxSplits = 64;
 
 struct Shape {
@@ -949,8 +949,12 @@ extern "C" int h3_window_attn(const void* q, const void* k, const void* v, void*
   p.group = (int)(n_heads / n_kv_heads);
   p.s_q = (int)s_q;
   p.s_kv = (int)s_kv;
-  p.left = (int)(left < 0 || left > kMaxPos ? kMaxPos : left);
-  p.right = causal ? 0 : (int)(right < 0 || right > kMaxPos ? kMaxPos : right);
+  // A side without a bound, or with one beyond every key, reaches from any row of the call (and from the unused rows of
+  // its last 256) over all keys: positions plus and minus it stay inside int32 wherever the call's positions lie.
+  const int64_t far_left = std::max<int64_t>(0, q_start + s_q + 2 * kBlockM);
+  const int64_t far_right = std::max<int64_t>(0, s_kv - q_start);
+  p.left = (int)(left < 0 ? far_left : std::min(left, far_left));
+  p.right = causal ? 0 : (int)(right < 0 ? far_right : std::min(right, far_right));
   p.sinks = (int)std::min(sinks, s_kv);
   p.causal = causal ? 1 : 0;
   p.q_start = (int)q_start;

@@ -271,3 +271,47 @@ def test_status_word_is_not_made_inside_a_capture(cuda_dev, monkeypatch):
     q = _rand((2, 3, D), 40, cuda_dev)
     with pytest.raises(O.H3Error):
         O.window_attention(q, q, q, 1, 1)
+
+
+FAR = 1 << 29  # the farthest position
+
+
+@pytest.mark.parametrize("s_q", [1, 3, 140, 300])
+@pytest.mark.parametrize("q_start,left,right,sinks,causal", [
+    (-FAR, None, None, 0, False), (-FAR, 7, None, 5, False), (-FAR, None, FAR, 0, False), (-FAR, None, 2 * FAR, 0, False),
+    (FAR, None, None, 0, False), (FAR, None, 0, 0, True), (FAR, FAR, 0, 9, True), (FAR, FAR - 40, 3, 0, False),
+    (FAR, 2 * FAR, 0, 0, True), (FAR, 100, 100, 0, False), (-FAR, 100, 100, 30, True)])
+def test_far_positions(cuda_dev, s_q, q_start, left, right, sinks, causal):
+    """Sides without a bound have none at the ends of the range of positions either, and bounds of 2^29 are exact."""
+    import h3attn as O
+    q, k, v = _rand((4, s_q, D), 50, cuda_dev), _rand((2, 1000, D), 51, cuda_dev), _rand((2, 1000, D), 52, cuda_dev)
+    for splits in (None, 1, 3):
+        o, (ref, mag) = _run(O, q, k, v, left, right, sinks, causal, q_start, splits=splits)
+        _check(o, ref, mag)
+
+
+def test_far_sides_through_the_c_entry(cuda_dev):
+    """The C call's own -1 and sides past 2^29, which the Python entry clips before."""
+    import h3attn as O
+    q, k, v = _rand((2, 40, D), 53, cuda_dev), _rand((2, 600, D), 54, cuda_dev), _rand((2, 600, D), 55, cuda_dev)
+    out = torch.empty_like(q)
+    st = O.status_word(cuda_dev)
+    for q_start, left, right, want in ((-FAR, -1, -1, (None, None)), (FAR, -1, 0, (None, 0)), (FAR, FAR + 20, 0, (FAR + 20, 0)),
+                                       (FAR, 1 << 62, 1 << 62, (None, None)), (-FAR, 0, FAR + 20, (0, FAR + 20))):
+        rc = O.lib().h3_window_attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 2, 2, 40, 600, 40 * D, D,
+                                    600 * D, D, 40, 0, 40 * D, D, D ** -0.5, left, right, 0, 0, q_start, 1, None, 0,
+                                    st.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        O.check_status()
+        _check(out, *_reference(q, k, v, *want, 0, False, q_start, 600))
+
+
+@pytest.mark.parametrize("group", [2, 5])
+def test_one_split_rows_do_not_depend_on_the_key_heads_of_the_call(cuda_dev, group):
+    """Query heads of any key heads of the call, with the same number of them to a key head."""
+    import h3attn as O
+    q = _rand((4 * group, 500, D), 56, cuda_dev)
+    k, v = (_rand((4, 500, D), 57 + i, cuda_dev) for i in range(2))
+    whole = O.window_attention(q, k, v, 100, 30, sinks=20, splits=1)
+    part = O.window_attention(q[group:3 * group], k[1:3], v[1:3], 100, 30, sinks=20, splits=1)
+    assert torch.equal(part, whole[group:3 * group])
