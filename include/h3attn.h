@@ -178,7 +178,8 @@ int h3_attn_fwd_peer(const void* q, const void* k, const void* v, void* o_local,
  *   at most 128 times it; query head h reads key head h / (n_heads / n_kv_heads)); o as h3_attn_fwd. Lengths and
  *   |q_start| up to 2^29.
  * splits: how many parts the key axis of a block of queries is worked in: 0 lets the call choose by its shape and the
- * GPU, 1 splits nothing (a query row's bits then do not depend on which heads share the call), up to 64.
+ * GPU, 1 splits nothing (a query row's bits then do not depend on how many key heads share the call, each with the same
+ * number of query heads), up to 64.
  * h3_window_attn_workspace returns the bytes of fp32 workspace that a call needs (16-byte aligned; 0: none), or an
  * error; it may be reused once the call's work on the stream is done. */
 int64_t h3_window_attn_workspace(int64_t n_heads, int64_t n_kv_heads, int64_t s_q, int64_t s_kv, int64_t left,

@@ -275,7 +275,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: in
     defaults to max(s_kv - Sq, 0): the queries are the last keys. A query that sees no key gets zeros. K and V
     may hold anything at keys that no query sees. out / layout / world as attention().
     splits: how many parts the key axis is worked in (None: chosen by the call's sizes); with 1 a query row's
-    bits do not depend on how many heads share the call."""
+    bits do not depend on how many key heads share the call, each with the same number of query heads."""
     for n, t in (("q", q), ("k", k), ("v", v)):
         _cuda(t, n)
         if t.dim() != 3 or t.shape[-1] != D or t.stride(-1) != 1:
