@@ -150,3 +150,27 @@ def near(a, b):
     """Two bf16 runs of the same blocks, or one and the fp32 model: every op rounds to bf16 (2^-8) some ten times a
     block, so the mean difference stays well below 2 % of the mean magnitude."""
     return (a - b).abs().mean().item() < 2e-2 * b.abs().mean().item()
+
+
+# A bf16 run against the fp32 model, row by row: every op of a block rounds to bf16, ten roundings in a row of them,
+# each off by at most 2^-8 of a value and by 2^-8 / sqrt(3) in the root mean square over a row. Two blocks, all errors
+# added at their full size: 20 * 2^-8 / sqrt(3) = 4.5 % of the row's length.
+ROW_BOUND = 20 * 2 ** -8 / math.sqrt(3)
+
+
+def row_errors(a, b):
+    """Relative L2 error of each token's row of a against b's."""
+    return (a - b).norm(dim=1) / b.norm(dim=1)
+
+
+def mistakes(S):
+    """Options that differ from setup(S)'s at a single token or key: segments and window edges one off."""
+    model, h, t_emb, segs, rope, stacks, options = setup(S, torch.device("cpu"))
+    w, (first, second, third) = options["h3_window"], options["h3_adapter_segments"]
+    changes = [{"h3_adapter_segments": s} for s in (
+        [(0, first[1] + 1, 2), (first[1] + 1, second[1], 0), third], [first, (40, second[1] - 1, 0), third],
+        [first, second, (third[0] + 1, S, 1)], [first, second, (third[0], S - 1, 1)])]
+    changes += [{"h3_window": dict(w, **{k: w[k] + d})} for k, d in (("sinks", -1), ("left", 1), ("right", 1))]
+    for change in changes:
+        with torch.no_grad():
+            yield change, plain(model, h, t_emb, segs, rope, stacks, dict(options, **change))

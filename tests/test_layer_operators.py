@@ -169,3 +169,18 @@ def test_projections_with_adapters_do_not_depend_on_the_shard(monkeypatch):
     finally:
         sp_runtime.uninstall()
     assert asked == [True] * 4
+
+
+@pytest.mark.parametrize("world", [1, 2, 4])
+def test_every_row_of_run_blocks(world, tmp_path):
+    """Row by row, so that one token with a neighbour's adapter, or a window one key off, shows -- which it does when
+    the mistake is made in the model that the run is compared with."""
+    S = 203
+    if world > 1:
+        T.run(1, S, tmp_path)  # leaves the fp32 model's output
+    got, ref = T.run(world, S, tmp_path), torch.load(tmp_path / "plain.pt")
+    for k in ("out", "dense"):
+        assert T.row_errors(got[k], ref[k]).max() < T.ROW_BOUND, k
+    if world == 1:
+        for change, wrong in T.mistakes(S):
+            assert T.row_errors(got["out"], wrong).max() > T.ROW_BOUND, change

@@ -38,3 +38,11 @@ def test_short_shards_with_adapters_across_gpus(world, tmp_path):
         one, many = T.run(1, S, tmp_path, on_gpu=True), T.run(world, S, tmp_path, on_gpu=True)
         for k in ("dense", "out"):
             assert torch.equal(many[k], one[k]), (S, k)
+
+
+@pytest.mark.parametrize("S", [203, 1001])
+def test_every_row_of_run_blocks(S, tmp_path):
+    got = T.run(1, S, tmp_path, on_gpu=True)
+    ref = torch.load(tmp_path / "plain.pt")
+    for k in ("out", "dense"):
+        assert T.row_errors(got[k], ref[k]).max() < T.ROW_BOUND, k
