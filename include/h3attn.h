@@ -295,6 +295,25 @@ int h3_wait_kat(const void* tile, int64_t limit_ns, int32_t* status, void* strea
  *   h3_tile_kat_pair_pv: o_out[256][128] = p[256][128] . v[128][128]   (CTA r: p rows 128r.., v cols 64r..) */
 int h3_tile_kat_pair_qk(const void* q, const void* k, float* s_out, int32_t* status, void* stream);
 int h3_tile_kat_pair_pv(const void* p, const void* v, float* o_out, int32_t* status, void* stream);
+/* Plans of the kernels beside the layer, computed on the host by the functions that the kernels run; they launch nothing
+ * and need no GPU. The lists fail with H3_ERR_WORKSPACE where they are too short.
+ *   h3_window_plan_kat: key tiles of each work item of an h3_window_attn call on a GPU of `sms` SMs; the number of rows of
+ *     eight int32: CTA, its round, key head, first query of the item, its part of the keys, first key of the tile, end
+ *     of the run, flags (1 first-token run, 2 / 4 masked for the item's first / second Q tile); an item without keys has
+ *     one row with first key -1. H3_ERR_UNSUPPORTED where the call takes the single-token kernel.
+ *   h3_window_mask_kat: bits[4] of the 128 keys from `key` on that query `query` sees (first_run: in the first-token run)
+ *   h3_adapters_deal_kat: how up to 64 rows of h3_gemm_adapters deal the 128-row tiles of w and the `chunks` groups of 64
+ *     stacked columns in use to CTAs; rows of six int32: CTA, tile, first and end k-block, the piece's number in the tile,
+ *     pieces of the tile. *tile_pieces: pieces of a tile that the workspace holds
+ *   h3_pack_ranks_kat: destination rank of each head in h3_qknorm_rope_pack_axes */
+int64_t h3_window_plan_kat(int64_t n_heads, int64_t n_kv_heads, int64_t s_q, int64_t s_kv, int64_t left, int64_t right,
+                           int64_t sinks, int32_t causal, int64_t q_start, int64_t splits, int32_t sms, int32_t* tiles,
+                           int64_t max_tiles);
+int h3_window_mask_kat(int64_t s_kv, int64_t left, int64_t right, int64_t sinks, int32_t causal, int64_t s_q,
+                       int64_t q_start, int64_t query, int64_t key, int32_t first_run, uint32_t* bits);
+int64_t h3_adapters_deal_kat(int64_t w_rows, int64_t n_kb, int64_t chunks, int32_t sms, int32_t* pieces,
+                             int64_t max_pieces, int64_t* tile_pieces);
+int h3_pack_ranks_kat(int64_t n_heads, int64_t heads_per_rank, int32_t* ranks);
 
 /* No counterpart in the reference. The single-GPU attention layer -- h3_qknorm_rope_pack into
  * head-major q/k/v, then h3_attn_fwd into token-major o -- for callers that cannot allocate device

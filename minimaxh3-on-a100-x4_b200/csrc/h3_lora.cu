@@ -494,6 +494,35 @@ __host__ __device__ inline int last_cta(int tile, int per_tile, int per_cta) {
   return int(((long long)(tile + 1) * per_tile - 1) / per_cta);
 }
 
+// The share [begin, end) of CTA `cta` of `ctas` in the list of all tiles' k-blocks.
+struct Share {
+  int per_cta;
+  long long begin, end;
+};
+__host__ __device__ inline Share share_of(int tiles, int per_tile, int cta, int ctas) {
+  const long long total = (long long)tiles * per_tile;
+  Share s;
+  s.per_cta = int((total + ctas - 1) / ctas);
+  const long long from = (long long)cta * s.per_cta;
+  s.begin = from < total ? from : total;
+  s.end = from + s.per_cta < total ? from + s.per_cta : total;
+  return s;
+}
+// A CTA's pieces, k-blocks [kb0, kb1) of a tile, from the last to the first: the start of a tile, whole ones, the end of one
+// with its chunks of B. The piece that ends at g; g becomes its begin.
+struct Piece {
+  int tile, kb0, kb1;
+};
+__host__ __device__ inline Piece piece_of(const Share& s, int per_tile, long long& g) {
+  Piece q;
+  q.tile = int((g - 1) / per_tile);
+  const long long base = (long long)q.tile * per_tile;
+  q.kb1 = int(g - base);
+  q.kb0 = int(s.begin > base ? s.begin - base : 0);
+  g = base + q.kb0;
+  return q;
+}
+
 constexpr int kStreamThreads = 256;  // TMA, MMA, 4 epilogue warps, 2 warps that write T
 constexpr int kFewChunks = kFewRows * (kMaxRank / 64);  // chunks in use at most
 
@@ -571,27 +600,14 @@ __global__ void __launch_bounds__(kStreamThreads, 2)
   const WaitCtx ctx{&sh.abort, f.status};
   const bool run = sh.abort == 0;
   const int per_tile = f.n_kb + sh.count;
-  const long long total = (long long)s.tiles * per_tile;
-  const int per_cta = int((total + gridDim.x - 1) / gridDim.x);
-  const long long g_begin = min(total, (long long)blockIdx.x * per_cta), g_end = min(total, g_begin + per_cta);
+  const Share mine = share_of(s.tiles, per_tile, int(blockIdx.x), int(gridDim.x));
+  const int per_cta = mine.per_cta;
+  const long long g_begin = mine.begin, g_end = mine.end;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     s.head[0] = per_tile;
     s.head[1] = per_cta;
   }
-  // the CTA's pieces, k-blocks [kb0, kb1) of a tile, from the last to the first: the start of a tile, whole ones, the
-  // end of one with its chunks of B
-  struct Piece {
-    int tile, kb0, kb1;
-  };
-  auto piece = [&](long long& g) {  // the piece that ends at g; g becomes its begin
-    Piece q;
-    q.tile = int((g - 1) / per_tile);
-    const long long base = (long long)q.tile * per_tile;
-    q.kb1 = int(g - base);
-    q.kb0 = int(max(0ll, g_begin - base));
-    g = base + q.kb0;
-    return q;
-  };
+  auto piece = [&](long long& g) { return piece_of(mine, per_tile, g); };
 
   if (warp == 0 && run) {
     const bool issuer = elect_one();
@@ -798,6 +814,13 @@ static int check_adapters(int64_t rank, int64_t n_adapters) {
   return n_adapters * rank > 64ll * kMaxChunks ? H3_ERR_SHAPE : H3_OK;
 }
 
+// CTAs of stream_kernel: two per SM, four k-blocks each at least (a CTA's piece costs its write and its read).
+static int stream_ctas(int tiles, int64_t n_kb, int sms) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>(2 * sms, tiles * n_kb / 4));
+}
+// Pieces of a tile that the workspace holds, whatever the chunks in use add.
+static int64_t most_pieces(int tiles, int ctas) { return (ctas + tiles - 1) / tiles + 2; }
+
 static int make_layout(int64_t m, int64_t n_kb, int64_t kc_blocks, int64_t w_rows, int64_t rank, int64_t n_adapters,
                        bool tiles, Layout& l) {
   l = {};
@@ -820,11 +843,9 @@ static int make_layout(int64_t m, int64_t n_kb, int64_t kc_blocks, int64_t w_row
   s.tiles = (int)((w_rows + 127) / 128);
   s.columns = 128ll * s.tiles;
   l.a_tiles = (int)((stacked + 127) / 128);
-  // two CTAs per SM, four k-blocks each at least (a CTA's piece costs its write and its read)
-  l.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(2 * sms, s.tiles * n_kb / 4));
+  l.ctas = stream_ctas(s.tiles, n_kb, sms);
   l.list_bytes = 256;
-  const int64_t most = (l.ctas + s.tiles - 1) / s.tiles + 2;  // pieces of a tile, whatever the chunks in use add
-  l.part_bytes = most * m * s.columns * (int64_t)sizeof(float);
+  l.part_bytes = most_pieces(s.tiles, l.ctas) * m * s.columns * (int64_t)sizeof(float);
   return H3_OK;
 }
 
@@ -876,6 +897,27 @@ extern "C" int64_t h3_gemm_adapters_workspace(int64_t m, int64_t a_chunks, int64
   if ((rc = make_layout(m, kc * a_chunks, kc, epilogue == 1 ? 2 * n_out : n_out, rank, n_adapters, tiles, l)) != H3_OK)
     return rc;
   return l.bytes();
+}
+
+extern "C" int64_t h3_adapters_deal_kat(int64_t w_rows, int64_t n_kb, int64_t chunks, int32_t sms, int32_t* pieces,
+                                        int64_t max_pieces, int64_t* tile_pieces) {
+  if (!pieces || !tile_pieces) return H3_ERR_NULL;
+  if (w_rows < 1 || w_rows > (1ll << 31) || n_kb < 1 || n_kb > (1ll << 21) || chunks < 0 || chunks > kFewChunks || sms < 1)
+    return H3_ERR_SHAPE;
+  const int tiles = (int)((w_rows + 127) / 128), per_tile = (int)(n_kb + chunks), ctas = stream_ctas(tiles, n_kb, sms);
+  *tile_pieces = most_pieces(tiles, ctas);
+  int64_t n = 0;
+  for (int c = 0; c < ctas; ++c) {
+    const Share share = share_of(tiles, per_tile, c, ctas);
+    for (long long g = share.end; g > share.begin; ++n) {
+      if (n >= max_pieces) return H3_ERR_WORKSPACE;
+      const Piece q = piece_of(share, per_tile, g);
+      const int first = first_cta(q.tile, per_tile, share.per_cta), last = last_cta(q.tile, per_tile, share.per_cta);
+      const int32_t row[6] = {c, q.tile, q.kb0, q.kb1, c - first, last - first + 1};
+      std::copy(row, row + 6, pieces + 6 * n);
+    }
+  }
+  return n;
 }
 
 extern "C" int h3_gemm_adapters(const void* a, int64_t m, int64_t a_chunks, int64_t a_chunk_cols,

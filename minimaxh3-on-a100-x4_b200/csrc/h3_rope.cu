@@ -178,9 +178,16 @@ struct PackOut {
   int heads_per_rank;
   unsigned rank_magic;  // ceil(2^32 / heads_per_rank): h / heads_per_rank = h * magic >> 32, h < 2^16, from 2 a rank on
 };
+__host__ __device__ __forceinline__ int rank_of_head(const PackOut& o, int h) {
+  return o.heads_per_rank == 1 ? h : int((unsigned long long)(unsigned)h * o.rank_magic >> 32);
+}
+__host__ __device__ __forceinline__ void split_heads(PackOut& o, int heads_per_rank) {
+  o.heads_per_rank = heads_per_rank;
+  o.rank_magic = (unsigned)(((1ull << 32) + heads_per_rank - 1) / heads_per_rank);
+}
 template <int kTensor>
 __device__ __forceinline__ __nv_bfloat16* pack_row(const PackOut& o, int h, long long tok) {
-  const int r = o.heads_per_rank == 1 ? h : int(__umulhi((unsigned)h, o.rank_magic)), hl = h - r * o.heads_per_rank;
+  const int r = rank_of_head(o, h), hl = h - r * o.heads_per_rank;
   return o.rank_base != nullptr
              ? reinterpret_cast<__nv_bfloat16*>(o.rank_base[r]) + kTensor * o.tensor_stride +
                    (long long)hl * o.head_stride + (o.row_offset + tok) * kHeadDim
@@ -310,8 +317,7 @@ static int pack_impl(const void* q, const void* k, const void* v, int64_t in_row
   in.w[0] = reinterpret_cast<const __nv_bfloat16*>(q_weight);
   in.w[1] = reinterpret_cast<const __nv_bfloat16*>(k_weight);
   in.eps = eps;
-  o.heads_per_rank = (int)heads_per_rank;
-  o.rank_magic = (unsigned)(((1ull << 32) + heads_per_rank - 1) / heads_per_rank);
+  split_heads(o, (int)heads_per_rank);
   int parts = 1, part_heads = 1, rc;
   if ((rc = head_parts(s_l, n_heads, parts, part_heads)) != H3_OK) return rc;
   pack_axes_kernel<<<grid_for(s_l * parts, kWarps, 1 << 20), 32 * kWarps, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
@@ -345,6 +351,15 @@ extern "C" int h3_rope_axes(const void* x, int64_t x_row_stride, int64_t x_head_
       reinterpret_cast<const __nv_bfloat16*>(x), x_row_stride, x_head_stride, ax,
       reinterpret_cast<__nv_bfloat16*>(out), out_row_stride, out_head_stride, s, (int)n_heads, parts, part_heads);
   return cudaGetLastError() == cudaSuccess ? H3_OK : H3_ERR_LAUNCH;
+}
+
+extern "C" int h3_pack_ranks_kat(int64_t n_heads, int64_t heads_per_rank, int32_t* ranks) {
+  if (!ranks) return H3_ERR_NULL;
+  if (n_heads < 1 || n_heads > 65535 || heads_per_rank < 1 || heads_per_rank > n_heads) return H3_ERR_SHAPE;
+  PackOut o = {};
+  split_heads(o, (int)heads_per_rank);
+  for (int h = 0; h < n_heads; ++h) ranks[h] = rank_of_head(o, h);
+  return H3_OK;
 }
 
 extern "C" int h3_qknorm_rope_pack_axes(const void* q, const void* k, const void* v, int64_t in_row_stride,

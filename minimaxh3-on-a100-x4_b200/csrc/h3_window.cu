@@ -56,14 +56,17 @@ struct Params {
   int* status;
 };
 
+// The plan of a call (walks, masks, the deal of work items) is written for host and device: h3_window_plan_kat shows it
+// to tests without a GPU.
+//
 // Key tiles of one CTA: a_tiles tiles of the first-token run, then the run that begins at b_start.
 struct Walk {
   int a_tiles, a_end, b_start, b_end, n;
-  __device__ __forceinline__ int base(int j) const { return j < a_tiles ? j * kBlockN : b_start + (j - a_tiles) * kBlockN; }
-  __device__ __forceinline__ int end(int j) const { return j < a_tiles ? a_end : b_end; }
+  __host__ __device__ __forceinline__ int base(int j) const { return j < a_tiles ? j * kBlockN : b_start + (j - a_tiles) * kBlockN; }
+  __host__ __device__ __forceinline__ int end(int j) const { return j < a_tiles ? a_end : b_end; }
 };
 
-__device__ __forceinline__ Walk make_walk(const Params& p, int p_first, int p_last) {
+__host__ __device__ __forceinline__ Walk make_walk(const Params& p, int p_first, int p_last) {
   Walk w;
   const int lo = max(0, p_first - p.left), hi = min(p.s_kv - 1, p_last + p.right);
   const int ns = p.causal ? max(0, min(p.sinks, p_last + 1)) : p.sinks;
@@ -80,7 +83,7 @@ __device__ __forceinline__ Walk make_walk(const Params& p, int p_first, int p_la
 // Block of queries and key head of CTA w. The ends: before the middle block first_mid - 1, first_mid - 2, ... and behind
 // it first_mid + n_mid, ... in turn, with the head running fastest (heads_turn) or, where that would spread the K and V in
 // use beyond the L2, slowest.
-__device__ __forceinline__ void block_of(const Params& p, int w, int& block, int& kvh) {
+__host__ __device__ __forceinline__ void block_of(const Params& p, int w, int& block, int& kvh) {
   const int mid = p.n_mid * p.kv_heads;
   if (w < mid) {
     kvh = w / p.n_mid;
@@ -101,21 +104,21 @@ struct Item {
   int kvh, i0, z;
   int j_lo, n_kv;
 };
-// Work item of this CTA in round r, or -1. Rounds alternate in direction: items are in descending length, so that a CTA's
-// long and short ones even out.
+// Work item of CTA `cta` of `ctas` in round r, or -1. Rounds alternate in direction: items come
+// longest first but for the two ends' taking turns, so that a CTA's long and short ones even out.
 template <int kTiles>
-__device__ __forceinline__ int rounds_of(const Params& p) {
+__host__ __device__ __forceinline__ int rounds_of(const Params& p) {
   return kTiles == 1 ? 1 : p.rounds;  // one Q tile: a CTA per item
 }
 template <int kTiles>
-__device__ __forceinline__ int item_of(const Params& p, int r) {
-  if (kTiles == 1) return int(blockIdx.x);
-  const int c = (r & 1) ? int(gridDim.x) - 1 - int(blockIdx.x) : int(blockIdx.x);
-  const int w = r * int(gridDim.x) + c;
+__host__ __device__ __forceinline__ int item_of(const Params& p, int r, int cta, int ctas) {
+  if (kTiles == 1) return cta;
+  const int c = (r & 1) ? ctas - 1 - cta : cta;
+  const int w = r * ctas + c;
   return w < p.n_items ? w : -1;
 }
 template <int kTiles>
-__device__ __forceinline__ Item make_item(const Params& p, int w, Walk& walk) {
+__host__ __device__ __forceinline__ Item make_item(const Params& p, int w, Walk& walk) {
   Item it;
   int block;
   it.z = w % p.splits;
@@ -131,7 +134,7 @@ template <int kTiles>
 __device__ __forceinline__ Item next_item(const Params& p, int& r, Walk& walk) {
   Item it = {};
   for (; r < rounds_of<kTiles>(p); ++r) {
-    const int w = item_of<kTiles>(p, r);
+    const int w = item_of<kTiles>(p, r, int(blockIdx.x), int(gridDim.x));
     if (w < 0) continue;
     it = make_item<kTiles>(p, w, walk);
     if (it.n_kv > 0) break;
@@ -140,11 +143,30 @@ __device__ __forceinline__ Item next_item(const Params& p, int& r, Walk& walk) {
 }
 
 // Bits e of a 32-key word whose keys lie in [a, b] or below n (all relative to the word's first key).
-__device__ __forceinline__ uint32_t visible_bits(int a, int b, int n) {
+__host__ __device__ __forceinline__ uint32_t visible_bits(int a, int b, int n) {
   const uint32_t ge = a <= 0 ? 0xffffffffu : (a > 31 ? 0u : 0xffffffffu << a);
   const uint32_t le = b < 0 ? 0u : (b >= 31 ? 0xffffffffu : (2u << b) - 1u);
   const uint32_t lt = n <= 0 ? 0u : (n > 31 ? 0xffffffffu : (1u << n) - 1u);
   return (ge & le) | lt;
+}
+
+// Keys of [lo, hi] and keys below ns: what the row at position pos sees, or (sees_all) what every row of [first, last] sees.
+struct Seen {
+  int lo, hi, ns;
+};
+__host__ __device__ __forceinline__ Seen sees(const Params& p, int pos) {
+  return {pos - p.left, min(pos + p.right, p.s_kv - 1), p.causal ? min(p.sinks, pos + 1) : p.sinks};
+}
+__host__ __device__ __forceinline__ Seen sees_all(const Params& p, int first, int last) {
+  return {last - p.left, min(first + p.right, p.s_kv - 1), p.causal ? min(p.sinks, first + 1) : p.sinks};
+}
+// Whether a key tile of the walk hides a key from some row. A separate first-token run has no window in it.
+__host__ __device__ __forceinline__ bool is_masked(const Seen& all, int key, bool first_run) {
+  return !(key + kBlockN <= all.ns || (!first_run && key >= all.lo && key + kBlockN - 1 <= all.hi));
+}
+// The row's window counted from the tile's first key: arguments of visible_bits for its first word.
+__host__ __device__ __forceinline__ Seen in_tile(const Seen& row, int key, bool first_run) {
+  return {first_run ? 1 << 20 : row.lo - key, row.hi - key, row.ns - key};
 }
 
 template <int kTiles>
@@ -378,18 +400,13 @@ __global__ void __launch_bounds__(Cfg<kTiles>::kThreads, Cfg<kTiles>::kCtasPerSm
     bool ok = run;
     int jg = 0, items = 0;
     for (int r = 0; ok && r < rounds_of<kTiles>(p); ++r) {
-      const int w = item_of<kTiles>(p, r);
+      const int w = item_of<kTiles>(p, r, int(blockIdx.x), int(gridDim.x));
       if (w < 0) continue;
       Walk walk;
       const Item item = make_item<kTiles>(p, w, walk);
       const int it0 = item.i0 + t * p.tile_pos;        // the tile's first query
       const int pos = p.q_start + it0 + row_pos;       // this row's key position
-      const int row_lo = pos - p.left, row_hi = min(pos + p.right, p.s_kv - 1);
-      const int row_ns = p.causal ? min(p.sinks, pos + 1) : p.sinks;
-      // what every row of the tile sees: keys below all_ns, keys of [all_lo, all_hi]
-      const int t_first = p.q_start + it0, t_last = t_first + p.tile_pos - 1;
-      const int all_lo = t_last - p.left, all_hi = min(t_first + p.right, p.s_kv - 1);
-      const int all_ns = p.causal ? min(p.sinks, t_first + 1) : p.sinks;
+      const Seen row = sees(p, pos), all = sees_all(p, p.q_start + it0, p.q_start + it0 + p.tile_pos - 1);
       float m_run = -INFINITY;
       uint64_t l_a = f2_pack(0.f, 0.f), l_b = f2_pack(0.f, 0.f);
 
@@ -406,19 +423,18 @@ __global__ void __launch_bounds__(Cfg<kTiles>::kThreads, Cfg<kTiles>::kCtasPerSm
         tc_fence_after();
         const int key = walk.base(item.j_lo + j);
         const bool first_run = item.j_lo + j < walk.a_tiles;
-        const bool masked = !(key + kBlockN <= all_ns ||
-                              (!first_run && key >= all_lo && key + kBlockN - 1 <= all_hi));
+        const bool masked = is_masked(all, key, first_run);
         uint32_t sa[64], sb[64];
         tmem_ld64_wait(tS, sa);
         tmem_ld64_nowait(tS + 64, sb);
         float s[128];
 #pragma unroll
         for (int i = 0; i < 64; ++i) s[i] = __uint_as_float(sa[i]);
-        const int ma = first_run ? 1 << 20 : row_lo - key, mb = row_hi - key, mn = row_ns - key;
+        const Seen at = in_tile(row, key, first_run);
         if (masked) {
 #pragma unroll
           for (int w = 0; w < 2; ++w) {
-            const uint32_t bits = visible_bits(ma - 32 * w, mb - 32 * w, mn - 32 * w);
+            const uint32_t bits = visible_bits(at.lo - 32 * w, at.hi - 32 * w, at.ns - 32 * w);
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (!((bits >> i) & 1u)) s[32 * w + i] = -INFINITY;
@@ -441,7 +457,7 @@ __global__ void __launch_bounds__(Cfg<kTiles>::kThreads, Cfg<kTiles>::kCtasPerSm
         if (masked) {
 #pragma unroll
           for (int w = 2; w < 4; ++w) {
-            const uint32_t bits = visible_bits(ma - 32 * w, mb - 32 * w, mn - 32 * w);
+            const uint32_t bits = visible_bits(at.lo - 32 * w, at.hi - 32 * w, at.ns - 32 * w);
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (!((bits >> i) & 1u)) s[32 * w + i] = -INFINITY;
@@ -818,10 +834,7 @@ struct Plan {
 // token_kernel, a CTA for 128 keys up to 8 of them. Else Q tiles of window_kernel: two per CTA (256 packed rows, one
 // CTA an SM) where the rows fill more than one, else one (two CTAs an SM); and splits only when the unsplit grid
 // leaves CTA slots empty: then as many as fill them, with at least two key tiles each.
-static int make_plan(const Shape& s, int64_t splits_asked, Plan& pl) {
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return H3_ERR_CUDA;
+static int make_plan(const Shape& s, int64_t splits_asked, int sms, Plan& pl) {
   const int group = (int)(s.n_heads / s.n_kv_heads);
   pl.tile_pos = 128 / group;
   pl.tiles = s.s_q <= pl.tile_pos ? 1 : 2;
@@ -861,6 +874,68 @@ static int make_plan(const Shape& s, int64_t splits_asked, Plan& pl) {
   // two tiles: a CTA per SM walks the items; one tile: a CTA per item (few rows: there are hardly more than fit)
   pl.ctas = pl.tiles == 2 ? std::min(pl.n_items, sms) : pl.n_items;
   return H3_OK;
+}
+
+static int sm_count(int& sms) {
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess &&
+                 cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess
+             ? H3_OK
+             : H3_ERR_CUDA;
+}
+
+// The fields of Params that the plan reads.
+static void plan_params(const Shape& s, const Plan& pl, Params& p) {
+  p.n_heads = (int)s.n_heads;
+  p.group = (int)(s.n_heads / s.n_kv_heads);
+  p.s_q = (int)s.s_q;
+  p.s_kv = (int)s.s_kv;
+  // A side without a bound, or with one beyond every key, reaches from any row of the call (and from the unused rows of
+  // its last 256) over all keys: positions plus and minus it stay inside int32 wherever the call's positions lie.
+  const int64_t far_left = std::max<int64_t>(0, s.q_start + s.s_q + 2 * kBlockM);
+  const int64_t far_right = std::max<int64_t>(0, s.s_kv - s.q_start);
+  p.left = (int)(s.left < 0 ? far_left : std::min(s.left, far_left));
+  p.right = s.causal ? 0 : (int)(s.right < 0 ? far_right : std::min(s.right, far_right));
+  p.sinks = (int)std::min(s.sinks, s.s_kv);
+  p.causal = s.causal ? 1 : 0;
+  p.q_start = (int)s.q_start;
+  p.tile_pos = pl.tile_pos;
+  p.blocks = pl.blocks;
+  p.first_mid = pl.first_mid;
+  p.n_mid = pl.n_mid;
+  p.kv_heads = (int)s.n_kv_heads;
+  p.heads_turn = pl.heads_turn;
+  p.splits = pl.splits;
+  p.n_items = pl.n_items;
+  p.rounds = (pl.n_items + pl.ctas - 1) / pl.ctas;
+}
+
+// Key tiles of every work item, eight int32 a tile: CTA, round, key head, first query, part, first key, end of its run,
+// bit 0 first-token run, bits 1 and 2 masked for the block's first and second Q tile. An item without keys has one
+// with first key -1.
+template <int kTiles>
+static int64_t list_tiles(const Params& p, int ctas, int32_t* out, int64_t most) {
+  int64_t n = 0;
+  for (int r = 0; r < rounds_of<kTiles>(p); ++r)
+    for (int c = 0; c < ctas; ++c) {
+      const int w = item_of<kTiles>(p, r, c, ctas);
+      if (w < 0) continue;
+      Walk walk;
+      const Item it = make_item<kTiles>(p, w, walk);
+      for (int j = 0; j < std::max(it.n_kv, 1); ++j, ++n) {
+        if (n >= most) return H3_ERR_WORKSPACE;
+        const bool any = it.n_kv > 0, first_run = any && it.j_lo + j < walk.a_tiles;
+        const int key = any ? walk.base(it.j_lo + j) : -1;
+        int flags = first_run;
+        for (int t = 0; any && t < kTiles; ++t) {
+          const int first = p.q_start + it.i0 + t * p.tile_pos;
+          flags |= int(is_masked(sees_all(p, first, first + p.tile_pos - 1), key, first_run)) << (1 + t);
+        }
+        const int32_t row[8] = {c, r, it.kvh, it.i0, it.z, key, any ? walk.end(it.j_lo + j) : -1, flags};
+        std::copy(row, row + 8, out + 8 * n);
+      }
+    }
+  return n;
 }
 
 static int64_t workspace_bytes(const Shape& s, const Plan& pl) {
@@ -915,8 +990,42 @@ extern "C" int64_t h3_window_attn_workspace(int64_t n_heads, int64_t n_kv_heads,
   if ((rc = check_shape(s)) != H3_OK) return rc;
   if (splits < 0 || splits > kMaxSplits) return H3_ERR_SHAPE;
   Plan pl;
-  if ((rc = make_plan(s, splits, pl)) != H3_OK) return rc;
+  int sms = 0;
+  if ((rc = sm_count(sms)) != H3_OK || (rc = make_plan(s, splits, sms, pl)) != H3_OK) return rc;
   return workspace_bytes(s, pl);
+}
+
+extern "C" int64_t h3_window_plan_kat(int64_t n_heads, int64_t n_kv_heads, int64_t s_q, int64_t s_kv, int64_t left,
+                                      int64_t right, int64_t sinks, int32_t causal, int64_t q_start, int64_t splits,
+                                      int32_t sms, int32_t* tiles, int64_t max_tiles) {
+  const Shape s = {n_heads, n_kv_heads, s_q, s_kv, left, right, sinks, q_start, causal};
+  int rc;
+  if (!tiles) return H3_ERR_NULL;
+  if ((rc = check_shape(s)) != H3_OK) return rc;
+  if (splits < 0 || splits > kMaxSplits || sms < 1) return H3_ERR_SHAPE;
+  Plan pl;
+  if ((rc = make_plan(s, splits, sms, pl)) != H3_OK) return rc;
+  if (pl.token > 0) return H3_ERR_UNSUPPORTED;
+  Params p = {};
+  plan_params(s, pl, p);
+  return pl.tiles == 2 ? list_tiles<2>(p, pl.ctas, tiles, max_tiles) : list_tiles<1>(p, pl.ctas, tiles, max_tiles);
+}
+
+extern "C" int h3_window_mask_kat(int64_t s_kv, int64_t left, int64_t right, int64_t sinks, int32_t causal,
+                                  int64_t s_q, int64_t q_start, int64_t query, int64_t key, int32_t first_run,
+                                  uint32_t* bits) {
+  const Shape s = {1, 1, s_q, s_kv, left, right, sinks, q_start, causal};
+  int rc;
+  if (!bits) return H3_ERR_NULL;
+  if ((rc = check_shape(s)) != H3_OK) return rc;
+  if (query < 0 || query >= s_q || key < 0 || key >= s_kv) return H3_ERR_SHAPE;
+  Plan pl;
+  if ((rc = make_plan(s, 1, 1, pl)) != H3_OK) return rc;
+  Params p = {};
+  plan_params(s, pl, p);
+  const Seen at = in_tile(sees(p, (int)(q_start + query)), (int)key, first_run != 0);
+  for (int w = 0; w < kBlockN / 32; ++w) bits[w] = visible_bits(at.lo - 32 * w, at.hi - 32 * w, at.ns - 32 * w);
+  return H3_OK;
 }
 
 extern "C" int h3_window_attn(const void* q, const void* k, const void* v, void* o, int64_t n_heads,
@@ -940,33 +1049,13 @@ extern "C" int h3_window_attn(const void* q, const void* k, const void* v, void*
       (n_heads > 1 && q_head_stride == 0) || (n_kv_heads > 1 && kv_head_stride == 0))
     return H3_ERR_STRIDE;
   Plan pl;
-  if ((rc = make_plan(s, splits, pl)) != H3_OK) return rc;
+  int sms = 0;
+  if ((rc = sm_count(sms)) != H3_OK || (rc = make_plan(s, splits, sms, pl)) != H3_OK) return rc;
   if (ws_bytes < workspace_bytes(s, pl)) return H3_ERR_WORKSPACE;
   if (pl.splits > 1 && !workspace) return H3_ERR_NULL;
 
-  Params p;
-  p.n_heads = (int)n_heads;
-  p.group = (int)(n_heads / n_kv_heads);
-  p.s_q = (int)s_q;
-  p.s_kv = (int)s_kv;
-  // A side without a bound, or with one beyond every key, reaches from any row of the call (and from the unused rows of
-  // its last 256) over all keys: positions plus and minus it stay inside int32 wherever the call's positions lie.
-  const int64_t far_left = std::max<int64_t>(0, q_start + s_q + 2 * kBlockM);
-  const int64_t far_right = std::max<int64_t>(0, s_kv - q_start);
-  p.left = (int)(left < 0 ? far_left : std::min(left, far_left));
-  p.right = causal ? 0 : (int)(right < 0 ? far_right : std::min(right, far_right));
-  p.sinks = (int)std::min(sinks, s_kv);
-  p.causal = causal ? 1 : 0;
-  p.q_start = (int)q_start;
-  p.tile_pos = pl.tile_pos;
-  p.blocks = pl.blocks;
-  p.first_mid = pl.first_mid;
-  p.n_mid = pl.n_mid;
-  p.kv_heads = (int)n_kv_heads;
-  p.heads_turn = pl.heads_turn;
-  p.splits = pl.splits;
-  p.n_items = pl.n_items;
-  p.rounds = (pl.n_items + pl.ctas - 1) / pl.ctas;
+  Params p = {};
+  plan_params(s, pl, p);
   p.scale_log2 = (float)((double)softmax_scale * 1.4426950408889634);
   p.o = reinterpret_cast<__nv_bfloat16*>(o);
   p.o_rank_rows = o_rank_rows;

@@ -107,6 +107,14 @@ def lib() -> ctypes.CDLL:
         L.h3_window_attn.argtypes = [vp] * 4 + [i64] * 12 + [f32, i64, i64, i64, ctypes.c_int32, i64, i64, vp, i64, i32p,
                                      vp]
         L.h3_window_attn.restype = ctypes.c_int
+        L.h3_window_plan_kat.argtypes = [i64] * 7 + [ctypes.c_int32, i64, i64, ctypes.c_int32, vp, i64]
+        L.h3_window_plan_kat.restype = i64
+        L.h3_window_mask_kat.argtypes = [i64] * 4 + [ctypes.c_int32] + [i64] * 4 + [ctypes.c_int32, vp]
+        L.h3_window_mask_kat.restype = ctypes.c_int
+        L.h3_adapters_deal_kat.argtypes = [i64, i64, i64, ctypes.c_int32, vp, i64, vp]
+        L.h3_adapters_deal_kat.restype = i64
+        L.h3_pack_ranks_kat.argtypes = [i64, i64, vp]
+        L.h3_pack_ranks_kat.restype = ctypes.c_int
         L.h3_rope_axes.argtypes = [vp, i64, i64, vp, ctypes.c_int32, i64, vp, vp, ctypes.c_int32, vp, i64, i64, i64,
                                    i64, vp]
         L.h3_rope_axes.restype = ctypes.c_int
