@@ -167,14 +167,13 @@ def _on(index: int):
 
 
 def _status_ptr(index: int) -> int:
-    """Address of the status word, made before the first launch that hands it out: zeroed on its stream, and not
-    inside a graph capture, whose pool would own it."""
+    """Address of the status word, made before the first launch that hands it out, and not inside a graph capture,
+    whose pool would own it."""
     st = _status.get(index)
     if st is None:
         if torch.cuda.is_current_stream_capturing():
             raise H3Error("call status_word() once before the first graph capture on this device")
         st = status_word(torch.device("cuda", index))
-        torch.cuda.current_stream().synchronize()
     return st.data_ptr()
 
 
@@ -184,6 +183,8 @@ def status_word(device=None) -> torch.Tensor:
     st = _status.get(dev.index)
     if st is None:
         st = torch.zeros(1, dtype=torch.int32, device=dev)
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(dev).synchronize()  # zero before a call on any other stream reads it
         _status[dev.index] = st
     return st
 

@@ -96,3 +96,16 @@ def test_runtime_raises_on_a_reported_failure(cuda_dev):
         assert torch.equal(good, again)
     finally:
         sp_runtime.uninstall()
+
+
+def test_status_word_is_zero_for_every_stream(cuda_dev, monkeypatch):
+    """Made on a busy stream, the word is zeroed before it is handed out: a kernel on another stream reads it at once, and
+    anything but zero would make it leave its output unwritten."""
+    import h3attn
+    monkeypatch.setattr(h3attn, "_status", {})
+    busy = torch.cuda.Stream()
+    with torch.cuda.stream(busy):
+        torch.cuda._sleep(200_000_000)  # a tenth of a second
+        st = h3attn.status_word(cuda_dev)
+    assert busy.query()
+    assert st.item() == 0
