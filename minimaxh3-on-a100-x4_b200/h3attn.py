@@ -190,9 +190,11 @@ def status_word(device=None) -> torch.Tensor:
 
 
 def check_status(device=None) -> None:
-    """Synchronise and raise if a kernel on `device` reported a bounded-wait timeout."""
+    """Synchronise with the stream that is current on `device` and raise if a kernel there reported a bounded-wait
+    timeout."""
     st = status_word(device)
-    code = lib().h3_status_read(ctypes.c_void_p(st.data_ptr()), ctypes.c_void_p(_stream()))
+    with _on(st.get_device()):
+        code = lib().h3_status_read(ctypes.c_void_p(st.data_ptr()), ctypes.c_void_p(_stream()))
     if code < 0:
         _check(code, "h3_status_read")
     if code != 0:

@@ -245,3 +245,35 @@ def test_row_independent_adapters_take_the_tiles(L):
     ok = [p, 20, 1, 512, 0, 512, p, 256, 512, p, 512, p, 64, 16, 4, p, p, p, 256, flag, p, 0, st, None]
     assert L.h3_gemm_adapters(*ok) == -12
     assert L.h3_gemm_adapters(*(ok[:19] + [flag | 2] + ok[20:])) == -3
+
+
+def test_status_is_read_on_its_devices_stream(monkeypatch):
+    """check_status(device) waits for the stream of that device, not of the current one (faked: no GPU)."""
+    import contextlib
+
+    import h3attn as O
+    current, read = [0], []
+
+    class Word:
+        get_device = staticmethod(lambda: 3)
+        data_ptr = staticmethod(lambda: 0x1000)
+
+    class Lib:
+        @staticmethod
+        def h3_status_read(status, stream):
+            read.append((status.value, stream.value))
+            return 0
+
+    @contextlib.contextmanager
+    def device(index):
+        before, current[0] = current[0], index
+        yield
+        current[0] = before
+
+    monkeypatch.setattr(O, "lib", Lib)
+    monkeypatch.setattr(O, "status_word", lambda device=None: Word)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(O, "_stream", lambda: 0x100 + current[0])
+    O.check_status(torch.device("cuda", 3))
+    assert read == [(0x1000, 0x103)] and current == [0]
