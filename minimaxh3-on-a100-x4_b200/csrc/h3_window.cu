@@ -827,13 +827,23 @@ struct Plan {
   int token;     // cluster size of token_kernel, or 0: window_kernel
 };
 
-// A single token with at most 4 query heads to a key head, over few keys, or over a cache with key heads enough that clusters of
-// 8 CTAs fill the SMs three times (fewer do not keep enough loads in flight): 1000 keys of 8 / 28 / 56 heads 4.8 / 5.8 /
-// 8.2 us, by tiles 9.8 / 10.7 / 13.2; 2000: 6.6 / 10.2 / 14.8 and 10.1 / 13.0 / 19.5; 4000: 10.2 / 20.9 / 25.3 and
-// 11.2 / 19.8 / 28.1; 8000: 31 / 36 / 43.7 and 15.6 / 28.0 / 45.3; 16000: 61 / 67 / 81.8 and 20.8 / 44 / 80.1. It is
-// token_kernel, a CTA for 128 keys up to 8 of them. Else Q tiles of window_kernel: two per CTA (256 packed rows, one
-// CTA an SM) where the rows fill more than one, else one (two CTAs an SM); and splits only when the unsplit grid
-// leaves CTA slots empty: then as many as fill them, with at least two key tiles each.
+// A single token with at most 4 query heads to a key head and few keys, or with a head of its own over a cache with key
+// heads enough that clusters of 8 CTAs fill the SMs three times (fewer do not keep enough loads in flight), is token_kernel,
+// a CTA for 128 keys up to 8 of them. One query head to a key head, 1000 keys of 8 / 28 / 56 heads: 7.6 / 8.7 / 10.7 us, by
+// tiles 10.6 / 11.8 / 14.8; 2000: 11.9 / 13.2 / 16.4 and 10.9 / 14.6 / 21.0; 4000 of 56 heads: 28.4 and 31.1; 8000: 47.2
+// and 47.2 (of 8 heads, with keys in the L2: 31 and 15.6). With 2 to 4 the sums of a key cost as many times the
+// arithmetic, and at 92-128 registers a thread only two CTAs fit an SM: a second round of clusters costs more than it
+// hides. Groups of 2 / 4, 750 keys of 40 heads (240 CTAs): 9.0 / 11.1 us, by tiles 12.0 / 12.1; 1000 keys of 37 heads (296
+// CTAs): 15.1 / 18.9 and 12.5 / 12.6; 8000 of 56: 69 / 87 and 47 / 48. Groups of 4 lose to the tiles from some 12 tiles of
+// keys on where they fit (20 heads, 1500 keys 13.0 and 12.0; 2000: 15.6 and 13.4; 4 heads: 8.7 / 10.4 and 10.4 / 10.4).
+// Else Q tiles of window_kernel: two per CTA (256 packed rows, one CTA an SM) where the rows fill more than one, else
+// one (two CTAs an SM); and splits only when the unsplit grid leaves CTA slots empty: then as many as fill them,
+// with at least two key tiles each.
+static bool by_tokens(int group, int64_t kv_heads, int64_t key_tiles, int sms) {
+  if (group == 1) return key_tiles <= 16 || (key_tiles <= 64 && kv_heads * kTokenMaxCluster >= 3 * sms);
+  const int64_t ctas = kv_heads * std::min<int64_t>(kTokenMaxCluster, key_tiles);
+  return group <= 4 && key_tiles <= 16 && group * key_tiles <= 48 && 4 * ctas <= 7 * sms;
+}
 static int make_plan(const Shape& s, int64_t splits_asked, int sms, Plan& pl) {
   const int group = (int)(s.n_heads / s.n_kv_heads);
   pl.tile_pos = 128 / group;
@@ -860,8 +870,7 @@ static int make_plan(const Shape& s, int64_t splits_asked, int sms, Plan& pl) {
   pl.heads_turn = s.n_kv_heads * std::min(span, s.s_kv) * 512 <= (256ll << 20);
   const int64_t key_tiles = (std::min(span, s.s_kv) + kBlockN - 1) / kBlockN;
   pl.token = 0;
-  if (splits_asked == 0 && s.s_q == 1 && group <= 4 &&
-      (key_tiles <= 16 || (key_tiles <= 64 && s.n_kv_heads * kTokenMaxCluster >= 3 * sms))) {
+  if (splits_asked == 0 && s.s_q == 1 && by_tokens(group, s.n_kv_heads, key_tiles, sms)) {
     pl.token = (int)std::max<int64_t>(1, std::min<int64_t>(kTokenMaxCluster, key_tiles));
     pl.splits = pl.n_items = pl.ctas = 1;
     return H3_OK;

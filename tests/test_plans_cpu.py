@@ -176,3 +176,16 @@ def test_rank_of_every_head(L):
             out, p = _ints(n)
             assert L.h3_pack_ranks_kat(n, per, p) == 0 and np.array_equal(out, np.arange(n) // per)
     assert L.h3_pack_ranks_kat(8, 2, None) == -1 and L.h3_pack_ranks_kat(0, 1, p) == -3 and L.h3_pack_ranks_kat(8, 9, p) == -3
+
+
+@pytest.mark.parametrize("group,kv_heads,keys,token", [
+    (1, 56, 8000, True), (1, 56, 8300, False), (1, 28, 2000, True), (1, 28, 2200, False), (1, 200, 2000, True),
+    (2, 28, 2000, True), (2, 32, 1000, True), (2, 37, 1000, False), (2, 56, 500, True), (2, 56, 1000, False), (2, 56, 8000, False),
+    (3, 8, 2000, True), (3, 40, 700, True), (3, 60, 700, False), (4, 20, 1500, True), (4, 20, 1600, False), (4, 100, 250, True),
+    (4, 100, 500, False), (4, 56, 4000, False), (5, 4, 100, False)])
+def test_which_single_tokens_leave_the_tiles(L, group, kv_heads, keys, token):
+    """Both sides of the rule, on 148 SMs."""
+    out, p = _ints((400000, 8))
+    n = L.h3_window_plan_kat(group * kv_heads, kv_heads, 1, keys, -1, 0, 0, 1, keys - 1, 0, 148, p, len(out))
+    assert (n == -8) == token
+    assert L.h3_window_plan_kat(group * kv_heads, kv_heads, 1, keys, -1, 0, 0, 1, keys - 1, 1, 148, p, len(out)) > 0
