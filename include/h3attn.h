@@ -195,7 +195,7 @@ int h3_window_attn(const void* q, const void* k, const void* v, void* o, int64_t
  * counterpart in the reference, whose rotary embedding is a table of matrices (harness/sp_runtime.py:93-99).
  *   pos: [s][n_axes] (pos_type: int32 or fp32), contiguous; n_axes 1..64
  *   inv_freq: fp64 [64], radians per unit position of pair i; axis: int32 [64], the axis that turns pair i
- *     (outside [0, n_axes): the pair keeps its values). Pair i is (x[i], x[i + 64]), as in h3_qknorm_rope_pack:
+ *     (outside [0, n_axes): the pair keeps its values, if finite). Pair i is (x[i], x[i + 64]), as in h3_qknorm_rope_pack:
  *       theta = pos[token][axis[i]] * inv_freq[i]
  *       out[i] = cos*x[i] - sin*x[i+64],  out[i+64] = sin*x[i] + cos*x[i+64]     (inverse != 0: -theta)
  *   Angles are formed in fp64 and reduced to a turn before fp32; rows are fp32 and rounded once to bf16.

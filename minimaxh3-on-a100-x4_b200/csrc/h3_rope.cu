@@ -1,7 +1,8 @@
 // Rotary positions over several axes (time, height, width, ...), computed from the positions:
 //   theta_i = pos[token][axis_i] * inv_freq_i                       (64 pairs i of a 128-element head)
 //   y_i = cos(theta_i) x_i - sin(theta_i) x_(i+64),  y_(i+64) = sin(theta_i) x_i + cos(theta_i) x_(i+64)
-// A pair whose axis is outside [0, n_axes) keeps its values. Two forms:
+// A pair whose axis is outside [0, n_axes) keeps its finite values (it is turned by 0: an infinity makes its partner NaN,
+// 0 * inf, as it does in every pair). Two forms:
 //   * rope_axes: rotates [tokens][heads][128] (inverse: the transposed rotation, its gradient)
 //   * pack_axes: per-head RMSNorm of q and k, rotation and the seq->head send layout in one pass, as
 //     qknorm_rope_pack does with a table of 2x2 matrices (1 KB per token, which this form does not read)
@@ -16,7 +17,8 @@
 // (or a share of its rows, when there are fewer tokens than warps): each lane evaluates two of the
 // 64 sine/cosine pairs, the warp exchanges them through shared memory, and its four 8-lane groups
 // take one head row each (16 elements a lane, 16-byte accesses, both halves of a pair in one lane),
-// two (pack) or four rows a group in flight. rope_axes: 89 us at 40868 tokens x 28 heads = 6.6 TB/s, the copy rate.
+// two (pack) or four rows a group in flight. rope_axes: 92 us at 40868 tokens x 28 heads = 6.4 TB/s, 0.97 of the
+// copy rate.
 #include "h3_rows.cuh"
 #include "h3attn.h"
 
@@ -203,7 +205,7 @@ struct PackIn {
 };
 
 // Two rows in flight a group and three CTAs (24 warps) an SM, 80 registers without spills: 588 us at 42000 tokens x 56
-// heads = 6.14 TB/s, 0.94 of the copy rate. Four rows at two CTAs: 639 us, two rows at four CTAs (spills): 585 us there
+// heads = 6.14 TB/s, 0.94 of the copy rate (605-613 on boxes whose copies are as much slower). Four rows at two CTAs: 639 us, two rows at four CTAs (spills): 585 us there
 // but 92 against 83 us at 5250 tokens, one row at five: 634 us. (Weights and angles in registers as fp32, four rows:
 // 720 us; parameter arrays indexed by a runtime tensor number, which go through local memory: 690 us.)
 constexpr int kPackRows = 2;                // head rows in flight per 8-lane group

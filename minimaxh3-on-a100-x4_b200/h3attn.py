@@ -356,7 +356,7 @@ _PAIRS = torch.Size([D // 2])
 class RopePositions:
     """Positions of tokens on several axes and the frequencies that turn them:
       pos: [tokens, axes] int32 or fp32; inv_freq: fp64 [64] radians per unit position of pair (i, i + 64);
-      axis: int32 [64], the axis of each pair (outside [0, axes): the pair keeps its values).
+      axis: int32 [64], the axis of each pair (outside [0, axes): the pair keeps its values, if finite).
     Accepted by qknorm_rope_pack / _peer in place of a table of rotation matrices, by rope_axes, and as
     sp_runtime's rope_freqs."""
 
