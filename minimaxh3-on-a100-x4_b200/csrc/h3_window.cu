@@ -7,7 +7,8 @@
 // tcgen05 S = Q K^T (SS form) and O += P V (TS form) on 128 x 128 tiles, one softmax thread per query
 // row, O rescaled only when a row maximum grew by more than 2^8, P rounded to bf16 for the second product
 // (the tensor cores' operand type: 2^-8 of a weight at most, averaged over a row's keys; the row sum keeps the
-// fp32 weights).
+// fp32 weights). Against 64 bits that is 2.3e-3 of the output; token_kernel, whose weights stay in fp32, is off by
+// 1.7e-3, the output's own rounding: a single token's error follows the kernel that its call takes.
 //
 // Tiles: the G = n_heads / n_kv_heads query heads that share a key head are packed into the rows of a Q
 // tile (row r = position r / G, head r % G), so a key tile is read once for all of them and a few query
@@ -20,16 +21,19 @@
 //
 // kTiles = 2: 256 packed rows a work item, 12 warps, 5-stage K/V ring, one CTA per SM (the full kernel's schedule). CTAs
 // are persistent: the ring runs on across items, the next item's Q loads once the last Q K^T of this one has retired, and
-// its first S is issued behind the last P V, so that only the write-back of O is left between two items (with a CTA
-// per item a start and an end cost 10 us of a 28 us item; 37 heads x 8192, window 511 + 512: 227 us, 206 so). kTiles = 1:
+// its first S is issued behind the last P V. An item costs 4.5 us beside its tiles so (the chain of its first tile, the
+// last P V, the write-back of O); with a CTA per item a start and an end cost 10 us of a 28 us item (37 heads x 8192,
+// window 511 + 512: 227 us, 206 so). kTiles = 1:
 // 128 packed rows, 8 warps, 2-stage ring, two CTAs per SM, a CTA per item. Few rows split the tile list over several
 // items; each writes (O, m, l) in fp32 to the caller's workspace and join_kernel combines them in a fixed order. A
 // single token has a kernel of its own (token_kernel).
 //
-// Bound: 42000 queries x 14 heads, window 2048 + 2048, 512 first tokens: 1.20 ms = 1122 TFLOP/s of visible pairs before
-// the power cap, 1.30-1.36 ms (1.0 PFLOP/s) under it; the exponentials and the chain S -> P -> O of a tile bound it, as in
-// the full kernel (1.85 us per 256 x 128 tile). A masked tile costs 0.09 us more. Short windows are bound by the walk's
-// start: 28 heads x 4096, window 511 + 512: 96 us. 5 tokens x 56 heads over 168000 keys of 8 heads: 116 us = 5.9 TB/s.
+// Bound: the exponentials and the chain S -> P -> O of a tile, as in the full kernel, at 1.97 us per 256 x 128 tile (the full
+// kernel: 1.88 on the same items), 0.09 us more where it is masked, and the 4.5 us an item. 42000 queries x 14 heads,
+// window 2048 + 2048, 512 first tokens: 1.34-1.40 ms under the power cap = 0.97-1.0 PFLOP/s of visible pairs, which are 95 %
+// of the tiles'; tensor and exponential pipes are 57 % busy on such a walk. 28 heads x 4096, window 511 + 512: 96-103 us,
+// pipes 43 % busy: 448 items for 148 CTAs leave one with 36 tiles in four items (71 + 18 us) where the mean is 30. 5 tokens x
+// 56 heads over 168000 keys of 8 heads: 113-130 us = 5.3-6.1 TB/s.
 #include <algorithm>
 #include <cmath>
 
@@ -645,7 +649,9 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const Params p, i
 // so there is nothing to mask, and a 128-row tile would be all padding. A cluster of CTAs takes the keys of one
 // key head, one run of them each; a half-warp takes a key (16 bytes of K and of V a lane), kKeys keys at a time in
 // flight, with its own running maximum and sums; half-warps join through shared memory, CTAs through distributed
-// shared memory. One launch, no workspace, and bound by the loads: 16 B x 2 x kKeys x 256 lanes a CTA in flight.
+// shared memory. One launch, no workspace, and bound by the latency of the loads: a half-warp asks for its next keys when
+// the sums of the ones before are done. 56 heads over 1536 of 42000 keys: three such rounds a CTA, 12 us with the keys in
+// the L2 and 14 without (44 MB: 3.1 TB/s); 23 % of the issue slots are used, ten warps wait on loads for each that issues.
 constexpr int kTokenWarps = 8;
 constexpr int kKeys = 4;  // keys in flight per half-warp
 constexpr int kTokenMaxCluster = 8;
