@@ -56,7 +56,9 @@ __device__ __forceinline__ int adapter_of(const Adapters& ad, int m, int r) {
 // cluster of kQuarters CTAs takes one part each (kCluster = 4) and the parts meet in distributed shared memory; with many, one
 // CTA takes them one after the other (kCluster = 1). Both give the same bits, so a row's T does not depend on the
 // call's length. One CTA per SM. 42000 rows of 7168: 99 us = 6.1 TB/s; whole calls of 1000 rows, 7168 -> 5376: 98 us with
-// one CTA per tile over all of k, 82 so; 65 rows of 5376 -> 21504, 4 adapters of rank 32: 86 and 77.
+// one CTA per tile over all of k, 82 so; 65 rows of 5376 -> 21504, 4 adapters of rank 32: 86 and 77. With many chunks in use
+// the launch is what bounds it: a tile's passes come one after the other, 43 us on 4 CTAs for 65 rows with 24 adapters of
+// rank 16 (two passes), 332 us on 32 CTAs for 1000 rows with 24 of rank 128 (twelve).
 constexpr int kQuarters = 4;
 constexpr uint32_t kChunkBytes = 64u * 64u * 2u;
 constexpr uint32_t kLowerRing = 192u * 1024u;
