@@ -13,8 +13,8 @@ Same module API and behaviour, B200 data path underneath:
   env SP_OVERLAP=heads         head-by-head all-to-all / attention pipelining (this build)
   env SP_OVERLAP=peer          all-to-alls fused into pack / attention over peer memory (this build)
   env SP_OVERLAP=ce            all-to-alls as copy-engine copies into peers' final buffers (this build)
-  rope_freqs                   may be an h3attn.RopePositions: rotary angles from (time, height, width) positions,
-                               computed inside the pack kernel (this build)
+  rope_freqs                   may be an h3attn.RopePositions of all tokens: rotary angles from (time, height, width)
+                               positions, computed inside the pack kernel (this build)
   transformer_options["h3_window"] = {"left": n, "right": n, "sinks": n}
                                attention over a sliding window, the first `sinks` tokens (the prompt) visible to all;
                                a missing or None side has no bound (this build; not with SP_OVERLAP=peer)
