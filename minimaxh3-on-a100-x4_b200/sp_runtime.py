@@ -236,7 +236,8 @@ def _check_adapters(model, segments, S) -> None:
         for part, forwards, names in (("attn", _ATTN_FORWARDS, ("qkv_proj", "out_proj")),
                                       ("mlp", (_sp_mlp_forward,), ("fc1", "fc2"))):
             part = getattr(blk, part, None)
-            if getattr(getattr(part, "forward", None), "__func__", None) in forwards:
+            # the patched class or one derived from it (whose own forward goes through the patched one)
+            if any(c.__dict__.get("forward") in forwards for c in type(part).__mro__):
                 routed.update(id(getattr(part, n, None)) for n in names)
     if any(id(m) not in routed for m in carrying):
         raise RuntimeError("sp_runtime: adapters are attached to a module that run_blocks does not apply them to "
@@ -780,7 +781,7 @@ def _sp_run_blocks(self, h, t_emb, mod_segments, rope_freqs, transformer_options
     _SP_ACTIVE, _SP_REAL_S = True, S
     seg_row = None
     try:
-        adapter_segs = (transformer_options or {}).get("h3_adapter_segments")
+        adapter_segs = list((transformer_options or {}).get("h3_adapter_segments") or ())
         if adapter_segs:
             _check_adapters(self, adapter_segs, S)
             _ADAPTER_ROWS = ops().segment_rows(_shard_segments(adapter_segs, lo, hi), h_loc.shape[0], h_loc.device)

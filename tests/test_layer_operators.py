@@ -184,3 +184,25 @@ def test_every_row_of_run_blocks(world, tmp_path):
     if world == 1:
         for change, wrong in T.mistakes(S):
             assert T.row_errors(got["out"], wrong).max() > T.ROW_BOUND, change
+
+
+def test_adapters_through_wrappers(monkeypatch):
+    """A forward that wraps the patched one, on the instance or in a subclass, still applies its adapters; segments may
+    be any iterable."""
+    import sp_runtime
+    S = 6
+    M, model, _ = _one_block(S, monkeypatch, S)
+    blk = model.blocks[0]
+    sp_runtime.set_adapters(blk.attn.qkv_proj, _adapters(blk.attn.qkv_proj, 2))
+    sp_runtime.set_adapters(blk.mlp.fc1, _adapters(blk.mlp.fc1, 2))
+    sp_runtime.install(M)
+    try:
+        bare, want = _run_adapted(M, model, S, []), _run_adapted(M, model, S, [(0, S, 1)])
+        assert not torch.equal(bare, want)
+        assert torch.equal(_run_adapted(M, model, S, iter([(0, S, 1)])), want)
+        inner = blk.attn.forward
+        blk.attn.forward = lambda *a, **k: inner(*a, **k)
+        blk.mlp.__class__ = type("Wrapped", (M.MLP,), {"forward": lambda self, x: M.MLP.forward(self, x)})
+        assert torch.equal(_run_adapted(M, model, S, [(0, S, 1)]), want)
+    finally:
+        sp_runtime.uninstall()
